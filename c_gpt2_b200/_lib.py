@@ -75,6 +75,16 @@ SIGNATURES = {
     "w8a8_attention_decode_workspace_reset": (_i, [_p, _sz, _p]),
     "w8a8_attention_decode_quant": (_i, [_p, _i64, _p, _p, _i64, _i, _p, _i, _i, _i, _p, _i64, _p,
                                          _p, _p, _sz, _p]),
+    "w8a8_pages_extend": (_i, [_p, _p, _p, _p]),
+    "w8a8_pages_write": (_i, [_p, _i, _p, _i64, _p, _i64, _i, _i, _p, _p, _p]),
+    "w8a8_pages_fork": (_i, [_p, _p, _p, _i, _p, _p]),
+    "w8a8_pages_free": (_i, [_p, _p, _i, _p]),
+    "w8a8_pages_compact_workspace_size": (_sz, [_i]),
+    "w8a8_pages_compact": (_i, [_p, _p, _p, _sz, _p]),
+    "w8a8_pages_copy": (_i, [_p, _p, _i64, _i, _p, _p, _i64, _i, _i64, _p, _p, _i, _p]),
+    "w8a8_attention_pages_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "w8a8_attention_pages": (_i, [_p, _i, _p, _i64, _i, _i, _p, _i, _p, _i, _i, _i, _p, _i64, _p,
+                                  _sz, _p]),
     "w8a8_lm_head": (_i, [_p, _i64, _i, _i, _p, _i, _p, _i64, _p]),
     "w8a8_sample_greedy": (_i, [_p, _i64, _i, _i, _p, _p, _i64, _p, _p]),
     "w8a8_sample_topk": (_i, [_p, _i64, _i, _i, _f, _i, _p, _i64, _p, _p, _p, _i64, _p, _p,
@@ -145,6 +155,13 @@ COMPAT_SIGNATURES = {
 class EngineConfig(C.Structure):
     _fields_ = [("d_model", _i), ("n_layer", _i), ("n_head", _i), ("vocab", _i), ("ctx", _i),
                 ("max_batch", _i), ("max_tokens", _i)]
+
+
+class Pages(C.Structure):
+    """w8a8_pages (include/gpt2_w8a8.h)."""
+    _fields_ = [("K", _p), ("V", _p), ("page_stride", _i64), ("n_pages", _i), ("page", _i),
+                ("n_layer", _i), ("n_kv_head", _i), ("table", _p), ("max_pages", _i),
+                ("n_slot", _i), ("n_ctx", _p), ("refs", _p)]
 
 
 class Request(C.Structure):

@@ -544,6 +544,175 @@ extern "C" int w8a8_attention_decode_quant(const gpt2_bf16_t *Q, int64_t ldq,
                                head_dim, O, ldo, Xq, sX, workspace, workspace_bytes, stream);
 }
 
+// Checks a page cache's description; the kernels' form of it in *a.
+static int pages_args(const w8a8_pages *c, PagesArgs *a) {
+  if (!c || !c->K || !c->V || !c->table || !c->n_ctx || !c->refs) return W8A8_ERR_INVALID;
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
+    return W8A8_ERR_UNSUPPORTED;
+  if (c->n_pages <= 0 || c->n_layer <= 0 || c->n_kv_head <= 0 || c->max_pages <= 0 ||
+      c->n_slot <= 0 || c->n_slot > W8A8_PAGES_MAX_LIST ||
+      (int64_t)c->n_slot * c->max_pages > 0x7fffffff)
+    return W8A8_ERR_INVALID;
+  // a page's 16-byte units are counted in 32 bits
+  const int64_t segs = (int64_t)c->n_layer * c->n_kv_head;
+  if (segs > (int64_t)0x7fffffff / (c->page * 16)) return W8A8_ERR_INVALID;
+  if (c->page_stride < segs * c->page * kPageHd || c->page_stride % 8 || !aligned16(c->K) ||
+      !aligned16(c->V))
+    return W8A8_ERR_INVALID;
+  int st;
+  DeviceCtx *ctx = device_ctx(&st);
+  if (!ctx) return st;
+  a->K = c->K;
+  a->V = c->V;
+  a->page_stride = c->page_stride;
+  a->n_pages = c->n_pages;
+  a->page = c->page;
+  a->n_layer = c->n_layer;
+  a->n_kv_head = c->n_kv_head;
+  a->table = c->table;
+  a->max_pages = c->max_pages;
+  a->n_slot = c->n_slot;
+  a->n_ctx = c->n_ctx;
+  a->refs = c->refs;
+  a->err = ctx->err;
+  return W8A8_OK;
+}
+
+static int sm_count(void) {
+  int st;
+  DeviceCtx *ctx = device_ctx(&st);
+  return ctx ? ctx->sm_count : 1;
+}
+
+extern "C" int w8a8_pages_extend(const w8a8_pages *c, const int32_t *n_new, int32_t *pos0,
+                                 void *stream) {
+  PagesArgs a;
+  if (!n_new || !pos0) return W8A8_ERR_INVALID;
+  int st = pages_args(c, &a);
+  if (st) return st;
+  return launch_pages_extend(a, n_new, pos0, (cudaStream_t)stream);
+}
+
+extern "C" int w8a8_pages_write(const w8a8_pages *c, int layer, const gpt2_bf16_t *Kn, int64_t ldk,
+                                const gpt2_bf16_t *Vn, int64_t ldv, int n_seq, int T,
+                                const int32_t *n_new, const int32_t *pos0, void *stream) {
+  PagesArgs a;
+  int st = pages_args(c, &a);
+  if (st) return st;
+  if (n_seq == 0 || T == 0) return W8A8_OK;
+  const int64_t d = (int64_t)a.n_kv_head * kPageHd;
+  if (!Kn || !Vn || !pos0 || layer < 0 || layer >= a.n_layer || n_seq < 0 || n_seq > a.n_slot ||
+      T < 0 || ldk < d || ldv < d || ldk % 8 || ldv % 8 || !aligned16(Kn) || !aligned16(Vn))
+    return W8A8_ERR_INVALID;
+  return launch_pages_write(a, layer, Kn, ldk, Vn, ldv, n_seq, T, n_new, pos0,
+                            (cudaStream_t)stream);
+}
+
+extern "C" int w8a8_pages_fork(const w8a8_pages *c, const int32_t *src, const int32_t *dst, int n,
+                               int32_t *status, void *stream) {
+  PagesArgs a;
+  int st = pages_args(c, &a);
+  if (st) return st;
+  if (n == 0) return W8A8_OK;
+  if (!src || !dst || !status || n < 0 || n > W8A8_PAGES_MAX_LIST) return W8A8_ERR_INVALID;
+  return launch_pages_fork(a, src, dst, n, status, sm_count(), (cudaStream_t)stream);
+}
+
+extern "C" int w8a8_pages_free(const w8a8_pages *c, const int32_t *slots, int n, void *stream) {
+  PagesArgs a;
+  int st = pages_args(c, &a);
+  if (st) return st;
+  if (n == 0) return W8A8_OK;
+  if (!slots || n < 0 || n > W8A8_PAGES_MAX_LIST) return W8A8_ERR_INVALID;
+  return launch_pages_free(a, slots, n, (cudaStream_t)stream);
+}
+
+extern "C" size_t w8a8_pages_compact_workspace_size(int n_pages) {
+  return n_pages <= 0 ? 0 : (3 * (size_t)n_pages + 1) * sizeof(int32_t);
+}
+
+extern "C" int w8a8_pages_compact(const w8a8_pages *c, int32_t *n_live, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+  PagesArgs a;
+  int st = pages_args(c, &a);
+  if (st) return st;
+  if (!n_live || !workspace || ((uintptr_t)workspace & 3) ||
+      workspace_bytes < w8a8_pages_compact_workspace_size(a.n_pages))
+    return W8A8_ERR_INVALID;
+  return launch_pages_compact(a, n_live, (int32_t *)workspace, sm_count(), (cudaStream_t)stream);
+}
+
+extern "C" int w8a8_pages_copy(const gpt2_bf16_t *Ksrc, const gpt2_bf16_t *Vsrc,
+                               int64_t src_stride, int n_src_pages, gpt2_bf16_t *Kdst,
+                               gpt2_bf16_t *Vdst, int64_t dst_stride, int n_dst_pages,
+                               int64_t page_elems, const int32_t *src, const int32_t *dst, int n,
+                               void *stream) {
+  if (n == 0) return W8A8_OK;
+  if (!Ksrc || !Vsrc || !Kdst || !Vdst || !src || !dst || n < 0 || n_src_pages <= 0 ||
+      n_dst_pages <= 0 || page_elems <= 0 || page_elems % 8 || src_stride < page_elems ||
+      dst_stride < page_elems || src_stride % 8 || dst_stride % 8 || !aligned16(Ksrc) ||
+      !aligned16(Vsrc) || !aligned16(Kdst) || !aligned16(Vdst))
+    return W8A8_ERR_INVALID;
+  int st;
+  DeviceCtx *ctx = device_ctx(&st);
+  if (!ctx) return st;
+  return launch_pages_copy(Ksrc, Vsrc, src_stride, n_src_pages, Kdst, Vdst, dst_stride,
+                           n_dst_pages, page_elems, src, dst, n, ctx->err, ctx->sm_count,
+                           (cudaStream_t)stream);
+}
+
+// Sizes that w8a8_attention_pages and its workspace size share.
+static bool attention_pages_sizes(int n_seq, int T, int n_head, int n_kv_head, int max_ctx,
+                                  int n_shared) {
+  return n_seq > 0 && T > 0 && n_head > 0 && n_kv_head > 0 && n_head % n_kv_head == 0 &&
+         max_ctx > 0 && max_ctx <= (1 << 30) && n_shared >= 0 && n_shared <= max_ctx &&
+         (int64_t)n_seq * T * n_head <= (1 << 30);
+}
+
+extern "C" size_t w8a8_attention_pages_workspace_size(int n_seq, int T, int n_head, int n_kv_head,
+                                                      int max_ctx, int n_shared) {
+  if (!attention_pages_sizes(n_seq, T, n_head, n_kv_head, max_ctx, n_shared)) return 0;
+  return attention_pages_workspace_bytes(n_seq, T, n_head, n_kv_head, max_ctx, n_shared);
+}
+
+extern "C" int w8a8_attention_pages(const w8a8_pages *c, int layer, const gpt2_bf16_t *Q,
+                                    int64_t ldq, int n_seq, int T, const int32_t *n_new,
+                                    int max_ctx, const int32_t *shared_pages, int n_shared,
+                                    int n_head, int head_dim, gpt2_bf16_t *O, int64_t ldo,
+                                    void *workspace, size_t workspace_bytes, void *stream) {
+  PagesArgs a;
+  int st = pages_args(c, &a);
+  if (st) return st;
+  if (n_seq == 0 || T == 0) return W8A8_OK;
+  if (head_dim != kPageHd) return W8A8_ERR_UNSUPPORTED;
+  if (!Q || !O || !workspace || layer < 0 || layer >= a.n_layer || n_seq > a.n_slot ||
+      !attention_pages_sizes(n_seq, T, n_head, a.n_kv_head, max_ctx, n_shared) ||
+      n_shared % a.page || (n_shared > 0 && !shared_pages))
+    return W8A8_ERR_INVALID;
+  const int64_t d = (int64_t)n_head * kPageHd;
+  if (ldq < d || ldo < d || ldq % 8 || ldo % 2 || !aligned16(Q) || ((uintptr_t)O & 3) ||
+      !aligned16(workspace) ||
+      workspace_bytes < attention_pages_workspace_bytes(n_seq, T, n_head, a.n_kv_head, max_ctx,
+                                                        n_shared))
+    return W8A8_ERR_INVALID;
+  AttnPagesCall q = {};
+  q.Q = Q;
+  q.ldq = ldq;
+  q.O = O;
+  q.ldo = ldo;
+  q.layer = layer;
+  q.n_seq = n_seq;
+  q.T = T;
+  q.n_head = n_head;
+  q.max_ctx = max_ctx;
+  q.n_shared = n_shared;
+  q.n_new = n_new;
+  q.shared = shared_pages;
+  q.ws = workspace;
+  q.ws_bytes = workspace_bytes;
+  return launch_attention_pages(a, q, sm_count(), (cudaStream_t)stream);
+}
+
 extern "C" int w8a8_lm_head(const gpt2_bf16_t *Xf, int64_t ldx, int M, int d,
                             const gpt2_bf16_t *wte, int V, gpt2_bf16_t *logits, int64_t ldl,
                             void *stream) {

@@ -204,4 +204,45 @@ int launch_topk_sample(const uint16_t *logits, int64_t ldl, int M, int V, float 
                        int32_t *out, int32_t *append_to, int64_t append_stride,
                        int32_t *append_pos, uint16_t *probs_out, int64_t ldp, cudaStream_t s);
 
+// Cache pages (w8a8_pages of include/gpt2_w8a8.h, with the device error word).
+constexpr int kPageHd = 64;  // head_dim of every pool
+struct PagesArgs {
+  uint16_t *K, *V;
+  int64_t page_stride;
+  int n_pages, page, n_layer, n_kv_head;
+  int32_t *table;
+  int max_pages, n_slot;
+  int32_t *n_ctx, *refs;
+  int *err;
+};
+// pages.cu
+int launch_pages_extend(const PagesArgs &a, const int32_t *n_new, int32_t *pos0, cudaStream_t s);
+int launch_pages_write(const PagesArgs &a, int layer, const uint16_t *Kn, int64_t ldk,
+                       const uint16_t *Vn, int64_t ldv, int n_seq, int T, const int32_t *n_new,
+                       const int32_t *pos0, cudaStream_t s);
+int launch_pages_fork(const PagesArgs &a, const int32_t *src, const int32_t *dst, int n,
+                      int32_t *status, int sm_count, cudaStream_t s);
+int launch_pages_free(const PagesArgs &a, const int32_t *slots, int n, cudaStream_t s);
+int launch_pages_compact(const PagesArgs &a, int32_t *n_live, int32_t *work, int sm_count,
+                         cudaStream_t s);
+int launch_pages_copy(const uint16_t *Ks, const uint16_t *Vs, int64_t src_stride, int n_src,
+                      uint16_t *Kd, uint16_t *Vd, int64_t dst_stride, int n_dst, int64_t elems,
+                      const int32_t *src, const int32_t *dst, int n, int *err, int sm_count,
+                      cudaStream_t s);
+// attention_pages.cu
+struct AttnPagesCall {
+  const uint16_t *Q;
+  int64_t ldq;
+  uint16_t *O;
+  int64_t ldo;
+  int layer, n_seq, T, n_head, max_ctx, n_shared;
+  const int32_t *n_new, *shared;
+  void *ws;
+  size_t ws_bytes;
+};
+size_t attention_pages_workspace_bytes(int n_seq, int T, int n_head, int n_kv_head, int max_ctx,
+                                       int n_shared);
+int launch_attention_pages(const PagesArgs &a, const AttnPagesCall &c, int sm_count,
+                           cudaStream_t s);
+
 }  // namespace w8a8

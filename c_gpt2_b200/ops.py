@@ -330,6 +330,157 @@ def attention_decode_quant(Q, Kc, Vc, seq_stride, n_ctx, max_ctx, n_head, worksp
     return O, Xq, sX
 
 
+# ---- cache pages (c_gpt2_b200/pages.py) ----
+
+def _here(t: torch.Tensor | None, dtype: torch.dtype, name: str, shape: tuple | None = None) -> int | None:
+    """Address of a contiguous tensor of this dtype (and shape) on the current device."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
+    """Address of bf16 rows [rows, cols] (row-strided) on the current device."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected {torch.bfloat16}, got {t.dtype}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device")
+    if tuple(t.shape) != (rows, cols) or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: expected [{rows}, {cols}] with contiguous rows")
+    return t.data_ptr()
+
+
+def _cache(cache):
+    if cache.device.type != "cuda" or cache.device.index != torch.cuda.current_device():
+        raise ValueError("cache: expected a cache on the current CUDA device")
+    return cache._ref
+
+
+def pages_extend(cache, n_new, pos0=None):
+    """Room for n_new[s] more positions of every slot s (int32 [n_slot]). Returns
+    pos0 [n_slot]: the first new position, -1 where none were asked for, -2 where
+    the pages did not suffice and the slot was left as it was."""
+    c = _cache(cache)
+    pos0 = pos0 if pos0 is not None else torch.empty_like(cache.n_ctx)
+    shape = (cache.n_slot,)
+    check(core().w8a8_pages_extend(c, _here(n_new, torch.int32, "n_new", shape),
+                                   _here(pos0, torch.int32, "pos0", shape), _stream()),
+          "w8a8_pages_extend")
+    return pos0
+
+
+def pages_write(cache, layer, K, V, pos0, T=1, n_new=None):
+    """Rows b*T + t of K, V [n_seq*T, n_kv_head*64] become position pos0[b] + t of
+    slot b's pages of this layer, for t < n_new[b] (default: all T), pos0[b] >= 0."""
+    c = _cache(cache)
+    n_seq, d = pos0.numel(), cache.n_kv_head * 64
+    shape = (n_seq,)
+    check(core().w8a8_pages_write(c, layer, _rows(K, n_seq * T, d, "K"), K.stride(0),
+                                  _rows(V, n_seq * T, d, "V"), V.stride(0), n_seq, T,
+                                  _here(n_new, torch.int32, "n_new", shape),
+                                  _here(pos0, torch.int32, "pos0", shape), _stream()),
+          "w8a8_pages_write")
+
+
+def pages_fork(cache, src, dst, status=None):
+    """Slot dst[i] (empty) goes on from slot src[i]. Returns status [n]: 0, or 1
+    where the entry named no such slots, one not empty or one named before, or 2
+    where no page was left; those entries did nothing."""
+    c = _cache(cache)
+    status = status if status is not None else torch.empty_like(src)
+    shape = (src.numel(),)
+    check(core().w8a8_pages_fork(c, _here(src, torch.int32, "src", shape),
+                                 _here(dst, torch.int32, "dst", shape), shape[0],
+                                 _here(status, torch.int32, "status", shape), _stream()),
+          "w8a8_pages_fork")
+    return status
+
+
+def pages_free(cache, slots):
+    """The slots (int32, device) give their pages back and are empty."""
+    c = _cache(cache)
+    check(core().w8a8_pages_free(c, _here(slots, torch.int32, "slots"), slots.numel(), _stream()),
+          "w8a8_pages_free")
+
+
+def pages_compact(cache, n_live=None, workspace=None):
+    """Moves the pages in use to the front of the pool; returns their number (int32
+    [1], device)."""
+    c = _cache(cache)
+    n_live = n_live if n_live is not None else torch.empty(1, dtype=torch.int32,
+                                                           device=cache.device)
+    if workspace is None:
+        workspace = torch.empty(core().w8a8_pages_compact_workspace_size(cache.n_pages),
+                                dtype=torch.uint8, device=cache.device)
+    check(core().w8a8_pages_compact(c, _here(n_live, torch.int32, "n_live", (1,)),
+                                    _here(workspace, torch.uint8, "workspace"),
+                                    workspace.numel(), _stream()), "w8a8_pages_compact")
+    return n_live
+
+
+def pages_copy(Ksrc, Vsrc, src, Kdst, Vdst, dst):
+    """Pages src[i] of the pools Ksrc, Vsrc to pages dst[i] of Kdst, Vdst (the first
+    dimension counts pages). The dst pages are distinct, and none is a source."""
+    n = src.numel()
+    size = Ksrc[0].numel()
+    for name, t in (("Ksrc", Ksrc), ("Vsrc", Vsrc), ("Kdst", Kdst), ("Vdst", Vdst)):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name}: expected {torch.bfloat16}, got {t.dtype}")
+        if not t.is_cuda or t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name}: expected a tensor on the current CUDA device")
+        if t.shape[1:] != Ksrc.shape[1:] or not t[0].is_contiguous():
+            raise ValueError(f"{name}: expected contiguous pages of {tuple(Ksrc.shape[1:])}")
+    if Ksrc.shape != Vsrc.shape or Ksrc.stride() != Vsrc.stride():
+        raise ValueError("Ksrc, Vsrc: expected the same shape and strides")
+    if Kdst.shape != Vdst.shape or Kdst.stride() != Vdst.stride():
+        raise ValueError("Kdst, Vdst: expected the same shape and strides")
+    ss = Ksrc.stride(0) if Ksrc.shape[0] > 1 else size
+    ds = Kdst.stride(0) if Kdst.shape[0] > 1 else size
+    check(core().w8a8_pages_copy(Ksrc.data_ptr(), Vsrc.data_ptr(), ss, Ksrc.shape[0],
+                                 Kdst.data_ptr(), Vdst.data_ptr(), ds, Kdst.shape[0], size,
+                                 _here(src, torch.int32, "src", (n,)),
+                                 _here(dst, torch.int32, "dst", (n,)), n, _stream()),
+          "w8a8_pages_copy")
+
+
+def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shared_pages=None,
+                    n_shared=0, out=None, workspace=None):
+    """Attention of the T newest positions of each sequence over its pages: rows
+    b*T + t of Q [n_seq*T, n_head*64] for t < n_new[b] (default: all T; the other
+    rows of the output are left as they were). The first n_shared positions are
+    read, once for the batch, from shared_pages (int32, device); max_ctx (default:
+    the table's) bounds every length."""
+    c = _cache(cache)
+    d = n_head * 64
+    n_seq = Q.shape[0] // T if T > 0 else 0
+    if max_ctx is None:
+        max_ctx = cache.max_pages * cache.page
+    if n_shared > 0 and (shared_pages is None or shared_pages.numel() * cache.page < n_shared):
+        raise ValueError("shared_pages: expected a page for every n_shared position")
+    q = _rows(Q, n_seq * T, d, "Q")
+    O = out if out is not None else torch.empty((n_seq * T, d), dtype=torch.bfloat16,
+                                                device=Q.device)
+    if workspace is None:
+        need = core().w8a8_attention_pages_workspace_size(n_seq, T, n_head, cache.n_kv_head,
+                                                          max_ctx, n_shared)
+        workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+    check(core().w8a8_attention_pages(c, layer, q, Q.stride(0), n_seq, T,
+                                      _here(n_new, torch.int32, "n_new", (n_seq,)), max_ctx,
+                                      _here(shared_pages, torch.int32, "shared_pages"), n_shared,
+                                      n_head, 64, _rows(O, n_seq * T, d, "out"), O.stride(0),
+                                      _here(workspace, torch.uint8, "workspace"),
+                                      workspace.numel(), _stream()), "w8a8_attention_pages")
+    return O
+
+
 def lm_head(Xf, wte):
     M, d = Xf.shape
     V = wte.shape[0]

@@ -252,6 +252,114 @@ int w8a8_attention_decode_quant(const gpt2_bf16_t *Q, int64_t ldq, const gpt2_bf
                                 gpt2_bf16_t *O, int64_t ldo, int8_t *Xq, float *sX,
                                 void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- cache pages (no counterpart in the reference, whose cache is one run of
+ * ctx rows per layer, gpt2.c:758-759) ----
+ * Sequences that go on from a common prompt hold its keys and values once. A
+ * page holds `page` positions of every layer:
+ *   row r of head h of layer l of page p:
+ *     K + p*page_stride + ((l*n_kv_head + h)*page + r)*64        (V alike)
+ * Slot s holds its first n_ctx[s] positions in the pages table[s*max_pages + k],
+ * k < ceil(n_ctx[s] / page); other entries are -1. refs[p] counts the slots
+ * that hold page p; a page with refs[p] == 0 is free. All of this is device
+ * memory of the caller: to begin, fill table with -1, n_ctx and refs with 0.
+ * The calls update it on the stream (they may be captured into a graph and
+ * replayed) and hand out free pages lowest index first, so the outcome is the
+ * same in every run. Calls on one cache must not overlap on the GPU.
+ *
+ * page is 16, 32, 64 or 128; n_slot and lists hold at most
+ * W8A8_PAGES_MAX_LIST entries; n_slot*max_pages < 2^31; pools are 16-byte
+ * aligned and page_stride >= n_layer*n_kv_head*page*64 is a multiple of 8
+ * elements. A table entry outside the pool is not followed: its position is
+ * skipped (attention reads zeros there) and recorded in the device error word. */
+typedef struct {
+  gpt2_bf16_t *K, *V;
+  int64_t page_stride; /* elements */
+  int32_t n_pages, page, n_layer, n_kv_head;
+  int32_t *table; /* [n_slot][max_pages] */
+  int32_t max_pages, n_slot;
+  int32_t *n_ctx; /* [n_slot] */
+  int32_t *refs;  /* [n_pages] */
+} w8a8_pages;
+
+#define W8A8_PAGES_MAX_LIST 8192
+#define W8A8_PAGES_NONE (-1)    /* w8a8_pages_extend: no tokens asked for */
+#define W8A8_PAGES_REFUSED (-2) /* w8a8_pages_extend: too few pages; nothing changed */
+#define W8A8_FORK_OK 0
+#define W8A8_FORK_BAD 1  /* no such slot, dst not empty, or named before in the list */
+#define W8A8_FORK_FULL 2 /* no page left for the source's last rows */
+
+/* Room for n_new[s] (device, [n_slot]) more positions of every slot s: n_ctx[s]
+ * grows by it, new pages join table and refs. pos0[s] (device, [n_slot])
+ * receives the first new position, W8A8_PAGES_NONE where n_new[s] <= 0, or
+ * W8A8_PAGES_REFUSED where the slot was left as it was: its table row is too
+ * short, or the free pages do not cover the pages that it and the slots before
+ * it ask for. */
+int w8a8_pages_extend(const w8a8_pages *c, const int32_t *n_new, int32_t *pos0, void *stream);
+
+/* Rows of a padded batch into the pages of one layer: row m = b*T + t of Kn and
+ * Vn (n_kv_head*64 wide, row strides ldk and ldv) becomes position pos0[b] + t
+ * of slot b < n_seq <= n_slot, for t < n_new[b] (n_new NULL: all T) and
+ * pos0[b] >= 0. Kn and Vn may be the K and V that w8a8_linear_qkv scatters with
+ * seq_stride T*n_kv_head*64 and pos0 NULL. */
+int w8a8_pages_write(const w8a8_pages *c, int layer, const gpt2_bf16_t *Kn, int64_t ldk,
+                     const gpt2_bf16_t *Vn, int64_t ldv, int n_seq, int T, const int32_t *n_new,
+                     const int32_t *pos0, void *stream);
+
+/* Slot dst[i] (empty) goes on from slot src[i], for i < n: it shares the whole
+ * pages, and the rows of a last, partly filled page are copied to a new one.
+ * Sources are read as they are before the call. status[i] (device, [n]) is
+ * W8A8_FORK_OK, or tells why the entry did nothing; pages run out in the order
+ * of the list. */
+int w8a8_pages_fork(const w8a8_pages *c, const int32_t *src, const int32_t *dst, int n,
+                    int32_t *status, void *stream);
+
+/* The slots slots[0..n) give their pages back and are empty. A slot may be
+ * named twice; indices outside [0, n_slot) are skipped. */
+int w8a8_pages_free(const w8a8_pages *c, const int32_t *slots, int n, void *stream);
+
+/* Moves the pages in use to the front of the pool: with n_live[0] of them (device,
+ * written), the j-th at index >= n_live goes to the j-th free index below, and
+ * the table follows. Pages from n_live on are free afterwards.
+ * workspace: w8a8_pages_compact_workspace_size(n_pages) bytes, any contents. */
+size_t w8a8_pages_compact_workspace_size(int n_pages);
+int w8a8_pages_compact(const w8a8_pages *c, int32_t *n_live, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Page src[i] of one pool pair to page dst[i] of another (or the same), i < n:
+ * page_elems (a multiple of 8) elements each of K and V. The dst pages are
+ * distinct, and none of them is a source. Indices outside the pools are skipped
+ * and recorded in the device error word. */
+int w8a8_pages_copy(const gpt2_bf16_t *Ksrc, const gpt2_bf16_t *Vsrc, int64_t src_stride,
+                    int n_src_pages, gpt2_bf16_t *Kdst, gpt2_bf16_t *Vdst, int64_t dst_stride,
+                    int n_dst_pages, int64_t page_elems, const int32_t *src, const int32_t *dst,
+                    int n, void *stream);
+
+/* ---- attention over the pages, a shared prefix read once ----
+ * T query rows a sequence, a padded batch: row m = b*T + t, head h reads
+ * Q[m*ldq + h*64 ..], for b < n_seq <= n_slot and t < n_new[b] (device, NULL:
+ * all T); slot b's n_ctx[b] positions include the new ones. Row t attends the
+ * positions below end = min(n_ctx[b], max_ctx) - n_new[b] + t + 1 of key head
+ * h / (n_head / n_kv_head):
+ *   O[m*ldo + h*64 ..] = bf16(softmax_j(q.k_j / 8) . V),  fp32 scores, maxima,
+ *   sums and accumulators; the weights are rounded to bf16 for the product with V.
+ * A row with end <= 0 is written as zeros; rows t >= n_new[b] are left as they
+ * were. Positions below n_shared (a multiple of page, at most max_ctx) are read
+ * from the n_shared / page pages shared_pages (device), for every sequence, and
+ * the table's entries for them are not read: with sequences forked from one
+ * prompt, any one's table row. Rows of pages that no query attends may hold
+ * anything; a value that is not finite at a position that some query attends
+ * may reach every query of the call that shares its key head.
+ * max_ctx bounds every n_ctx[b]. The workspace (any contents) is sized with
+ * w8a8_attention_pages_workspace_size; 16-byte aligned Q, ldq % 8 == 0, O
+ * 4-byte aligned, ldo even; n_head % n_kv_head == 0, head_dim 64. */
+size_t w8a8_attention_pages_workspace_size(int n_seq, int T, int n_head, int n_kv_head,
+                                           int max_ctx, int n_shared);
+int w8a8_attention_pages(const w8a8_pages *c, int layer, const gpt2_bf16_t *Q, int64_t ldq,
+                         int n_seq, int T, const int32_t *n_new, int max_ctx,
+                         const int32_t *shared_pages, int n_shared, int n_head, int hd,
+                         gpt2_bf16_t *O, int64_t ldo, void *workspace, size_t workspace_bytes,
+                         void *stream);
+
 /* ---- LM head (gpt2.c:2160): logits[M,V] = bf16(Xf[M,d] · wte[V,d]^T), fp32
  * accumulation. wte is used as stored ([vocab, d], K-major); the reference's
  * host transpose wte_T (gpt2.c:1915-1918) is not needed. */

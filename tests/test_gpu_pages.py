@@ -1,0 +1,533 @@
+"""GPU tests of the cache pages and of the attention that reads them."""
+import numpy as np
+import pytest
+import torch
+
+from c_gpt2_b200 import _lib, ops
+from c_gpt2_b200.pages import PageCache
+from tests import pages_oracle as po
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(a, device="cuda:0"):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device=device)
+
+
+def make(cuda, n_pages, n_slot, max_pages, n_layer=2, n_kv=3, page=16, seed=0):
+    """A cache whose pools hold random values (so that a row that should not have
+    been touched shows), and its oracle."""
+    c = PageCache.empty(n_pages, n_slot, max_pages, n_layer, n_kv, page, cuda)
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    for t in (c.K, c.V):
+        t.copy_(torch.randn(t.shape, generator=g, device=cuda))
+    return c, po.Book(n_slot, max_pages, n_pages, page)
+
+
+def same_book(c, b):
+    np.testing.assert_array_equal(c.table.cpu().numpy(), b.table)
+    np.testing.assert_array_equal(c.n_ctx.cpu().numpy(), b.n_ctx)
+    np.testing.assert_array_equal(c.refs.cpu().numpy(), b.refs)
+
+
+def apply_moves(K, V, moves):
+    for f, t, rows in moves:
+        K[t, :, :, :rows] = K[f, :, :, :rows]
+        V[t, :, :, :rows] = V[f, :, :, :rows]
+
+
+# ---- bookkeeping ------------------------------------------------------------
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_any_series_of_calls_keeps_the_oracle_books(cuda, page):
+    rng = np.random.default_rng(page)
+    n_slot = 7
+    c, b = make(cuda, 23, n_slot, 6, n_layer=1, n_kv=2, page=page)
+    K, V = c.K.clone(), c.V.clone()
+    for _ in range(60):
+        kind = rng.integers(5)
+        if kind <= 1:
+            n_new = rng.integers(-1, 3 * page, n_slot) * rng.integers(0, 2, n_slot)
+            pos0 = ops.pages_extend(c, i32(n_new))
+            np.testing.assert_array_equal(pos0.cpu().numpy(), b.extend(n_new))
+        elif kind == 2:
+            src, dst = rng.integers(-1, n_slot + 1, 4), rng.integers(-1, n_slot + 1, 4)
+            status = ops.pages_fork(c, i32(src), i32(dst))
+            want, moves = b.fork(src, dst)
+            np.testing.assert_array_equal(status.cpu().numpy(), want)
+            apply_moves(K, V, moves)
+        elif kind == 3:
+            slots = rng.integers(-1, n_slot + 1, 3)
+            ops.pages_free(c, i32(slots))
+            b.free(slots)
+        else:
+            n = ops.pages_compact(c)
+            want, moves = b.compact()
+            assert n.item() == want
+            apply_moves(K, V, moves)
+        same_book(c, b)
+    assert torch.equal(c.K, K) and torch.equal(c.V, V)
+
+
+@pytest.mark.parametrize("n_pages,n_slot", [(1, 1), (8191, 33), (8193, 1500), (40000, 8192)])
+def test_pages_over_several_rounds_of_a_scan(cuda, n_pages, n_slot):
+    """More pages than one round of a scan, more slots than threads, free pages few
+    and far between; then all at once until the pool runs out."""
+    rng = np.random.default_rng(n_pages)
+    c, b = make(cuda, n_pages, n_slot, 9, n_layer=1, n_kv=1)
+    b.refs[:] = rng.random(n_pages) < 0.9
+    b.refs[-1] = 0
+    c.refs.copy_(i32(b.refs))
+    for _ in range(3):
+        n_new = rng.integers(0, 60, n_slot)
+        np.testing.assert_array_equal(ops.pages_extend(c, i32(n_new)).cpu().numpy(),
+                                      b.extend(n_new))
+        same_book(c, b)
+    if n_slot > 1:
+        src, dst = rng.integers(0, n_slot, n_slot), rng.permutation(n_slot)
+        gone = dst[: n_slot // 2]
+        ops.pages_free(c, i32(gone))
+        b.free(gone)
+        same_book(c, b)
+        status = ops.pages_fork(c, i32(src), i32(dst))
+        np.testing.assert_array_equal(status.cpu().numpy(), b.fork(src, dst)[0])
+        same_book(c, b)
+    assert ops.pages_compact(c).item() == b.compact()[0]
+    same_book(c, b)
+
+
+def test_extend_refuses_as_a_whole(cuda):
+    """The pool ends inside the first slot's second request: it and the next two get
+    nothing, the fourth needs no page and is served; and a row too short."""
+    c, b = make(cuda, 5, 4, 4)
+    for n_new in ([16, 1, 1, 10], [20, 40, 16, 3], [1, 1, 1, 1], [0, -3, 0, 64]):
+        got = ops.pages_extend(c, i32(n_new)).cpu().numpy()
+        np.testing.assert_array_equal(got, b.extend(n_new))
+        same_book(c, b)
+    assert list(b.n_ctx) == [17, 2, 2, 14]
+
+
+def test_fork_runs_out_of_pages_in_list_order(cuda):
+    c, b = make(cuda, 4, 6, 4)
+    ops.pages_extend(c, i32([17, 0, 0, 0, 0, 0]))
+    b.extend([17, 0, 0, 0, 0, 0])
+    src, dst = [0, 0, 0, 0, 9], [5, 1, 3, 1, 2]
+    K, V = c.K.clone(), c.V.clone()
+    status = ops.pages_fork(c, i32(src), i32(dst)).cpu().numpy()
+    want, moves = b.fork(src, dst)
+    np.testing.assert_array_equal(status, want)
+    assert list(want) == [0, 0, 2, 1, 1]
+    same_book(c, b)
+    apply_moves(K, V, moves)
+    assert torch.equal(c.K, K) and torch.equal(c.V, V)
+    # given back, named twice and out of range: each page is counted down once
+    ops.pages_free(c, i32([5, 5, -1, 6, 0]))
+    b.free([5, 0])
+    same_book(c, b)
+    assert b.refs.sum() == 2
+
+
+def test_bad_entries_are_skipped_and_recorded(cuda):
+    """Table entries outside the pool: nothing is followed, the error word is set."""
+    for bad in (-7, 5, 2 ** 31 - 1):
+        c, _ = make(cuda, 5, 3, 3)
+        ops.pages_extend(c, i32([40, 0, 0]))
+        c.table[0, 1] = bad
+        refs = c.refs.clone()
+        assert ops.device_error() == 0
+        ops.pages_fork(c, i32([0]), i32([1]))
+        assert ops.device_error() == 0x1501
+        refs[0] += 1
+        refs[3] += 1  # the copied last page
+        assert torch.equal(c.refs, refs)
+        ops.pages_free(c, i32([0, 1]))
+        assert ops.device_error() == 0x1501
+        assert c.refs.tolist() == [0, 1, 0, 0, 0]
+    ops.pages_copy(c.K, c.V, i32([0, 5, -1]), c.K, c.V, i32([1, 2, 3]))
+    assert ops.device_error() == 0x1501
+    x = torch.zeros(3, 192, dtype=torch.bfloat16, device=cuda)
+    ops.pages_write(c, 0, x, x, i32([48, -1, -2]))
+    assert ops.device_error() == 0x1502  # behind the table
+    ops.pages_write(c, 0, x, x, i32([0, -1, -2]))
+    assert ops.device_error() == 0x1501  # no page there
+
+
+# ---- contents ---------------------------------------------------------------
+
+@pytest.mark.parametrize("T,page,strided", [(1, 16, True), (5, 16, False), (70, 32, True),
+                                            (200, 128, False)])
+def test_write_places_the_rows(cuda, T, page, strided):
+    n_seq, n_kv, n_layer = 4, 3, 3
+    c, b = make(cuda, 60, 5, 14, n_layer, n_kv, page, seed=T)
+    first = [0, 3, page, 2 * page - 1, 0]
+    ops.pages_extend(c, i32(first))
+    b.extend(first)
+    n_new = [T, 1, 0, max(T - 1, 1), 0]
+    pos0 = ops.pages_extend(c, i32(n_new))
+    b.extend(n_new)
+    same_book(c, b)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    rows = torch.randn(n_seq * T, 3 * n_kv * 64, generator=g, device=cuda).bfloat16()
+    d = n_kv * 64
+    Kn, Vn = (rows[:, d:2 * d], rows[:, 2 * d:]) if strided else (rows[:, d:2 * d].contiguous(),
+                                                                  rows[:, 2 * d:].contiguous())
+    K, V = c.K.clone(), c.V.clone()
+    ops.pages_write(c, 1, Kn, Vn, pos0[:n_seq], T=T, n_new=i32(n_new[:n_seq]))
+    for s in range(n_seq):
+        for t in range(n_new[s]):
+            pos = first[s] + t
+            p = b.table[s, pos // page]
+            K[p, 1, :, pos % page] = Kn[s * T + t].view(n_kv, 64)
+            V[p, 1, :, pos % page] = Vn[s * T + t].view(n_kv, 64)
+    assert torch.equal(c.K, K) and torch.equal(c.V, V)
+
+
+@pytest.mark.parametrize("shape", [(9, 1, 1, 16), (40, 5, 3, 32), (12, 36, 20, 32)])
+def test_copy_between_pools(cuda, shape):
+    """Pools of other sizes and strides; pages that are not named stay as they are."""
+    n, L, G, page = shape
+    g = torch.Generator(device=cuda).manual_seed(n)
+    kv = torch.randn(n, 2, L, G, page, 64, generator=g, device=cuda).bfloat16()
+    K2 = torch.randn(n + 3, L, G, page, 64, generator=g, device=cuda).bfloat16()
+    V2 = torch.randn(n + 3, L, G, page, 64, generator=g, device=cuda).bfloat16()
+    src, dst = torch.randperm(n)[: n - 1], torch.randperm(n + 3)[: n - 1]
+    wk, wv = K2.clone(), V2.clone()
+    wk[dst.cuda()], wv[dst.cuda()] = kv[src.cuda(), 0], kv[src.cuda(), 1]
+    ops.pages_copy(kv[:, 0], kv[:, 1], i32(src), K2, V2, i32(dst))
+    assert torch.equal(K2, wk) and torch.equal(V2, wv)
+
+
+# ---- attention --------------------------------------------------------------
+
+def build(cuda, n_seq, T, H, G, page, n_shared, tails, n_new, seed, n_layer=2, layer=1, scale=1.5,
+          junk=float("nan")):
+    """A cache with these tails behind a shared prefix, its unused rows filled with
+    `junk`; Q; and (O, A) of the 64-bit oracle for every sequence."""
+    rng = np.random.default_rng(seed)
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    ns = n_shared // page
+    per = [-(-t // page) for t in tails]
+    n_pages = ns + sum(per) + 3
+    order = rng.permutation(n_pages)
+    table = np.full((n_seq, ns + max(per + [1])), -1, np.int32)
+    at = ns
+    for b in range(n_seq):
+        if tails[b] >= 0:
+            table[b, :ns] = order[:ns]
+            table[b, ns:ns + per[b]] = order[at:at + per[b]]
+            at += per[b]
+    n_ctx = [n_shared + t if t >= 0 else 0 for t in tails]
+    shape = (n_pages, n_layer, G, page, 64)
+    K = torch.full(shape, junk, dtype=torch.bfloat16, device=cuda)
+    V = torch.full(shape, junk, dtype=torch.bfloat16, device=cuda)
+    for b in range(n_seq):
+        for k in range(-(-n_ctx[b] // page)):
+            rows = min(page, n_ctx[b] - k * page)
+            if k < ns and b != next(i for i in range(n_seq) if tails[i] >= 0):
+                continue
+            for pool in (K, V):
+                pool[table[b, k], :, :, :rows] = torch.randn(
+                    n_layer, G, rows, 64, generator=g, device=cuda).bfloat16()
+    Q = (torch.randn(n_seq * T, H * 64, generator=g, device=cuda) * scale).bfloat16()
+    c = PageCache(K, V, i32(table), i32(n_ctx), i32(np.ones(n_pages)))
+    want = []
+    k64, v64 = K[:, layer].double().cpu().numpy(), V[:, layer].double().cpu().numpy()
+    q64 = Q.double().cpu().numpy().reshape(n_seq, T, H, 64)
+    for b in range(n_seq):
+        p = table[b, :-(-n_ctx[b] // page)]
+        kb = k64[p].transpose(0, 2, 1, 3).reshape(-1, G, 64)[:n_ctx[b]]
+        vb = v64[p].transpose(0, 2, 1, 3).reshape(-1, G, 64)[:n_ctx[b]]
+        want.append(po.attention(q64[b], kb, vb, n_new[b]))
+    return c, Q, i32(order[:ns]) if ns else None, want
+
+
+def check(out, want, T, H, n_new, before=7.0):
+    """Against the 64-bit oracle. Roundings: the output (half a step, 2^-8 of its
+    value), each weight before the product with V (2^-8 of it at most, so 2^-8 of
+    A = sum w |V|), and the 32-bit scores, exponentials and sums, for which 2^-11 of
+    A is ample (a score of 64 products, |s| < 100: 2^-24 * 64 * 100 = 2^-11.4)."""
+    got = out.double().cpu().numpy().reshape(len(want), T, H, 64)
+    for b, (O, A) in enumerate(want):
+        tol = 2.0 ** -8 * np.abs(O) + (2.0 ** -8 + 2.0 ** -11) * A
+        err = np.abs(got[b, :n_new[b]] - O)
+        assert (err <= tol).all(), (b, float((err - tol).max()))
+        assert (got[b, n_new[b]:] == before).all(), "rows behind a sequence's last were touched"
+
+
+CASES = [
+    # n_seq, T, H, G, page, n_shared, tails
+    (1, 1, 1, 1, 16, 0, [1]),
+    (1, 1, 12, 12, 16, 0, [17]),
+    (2, 1, 12, 12, 16, 64, [5, 32]),
+    (3, 1, 4, 2, 32, 32, [0, 1, 65]),                # a tail of zero: all in the prefix
+    (5, 1, 6, 3, 16, 16, [-1, 7, -1, 130, 64]),      # empty sequences among others
+    (9, 1, 7, 1, 64, 640, [3, 64, 65, 100, 1, 2, 700, 128, 127]),
+    (33, 1, 4, 4, 128, 1280, list(range(1, 34))),
+    (70, 1, 2, 1, 16, 304, [1 + 5 * i for i in range(70)]),
+    (150, 1, 2, 2, 32, 96, [1 + i % 40 for i in range(150)]),
+    (2, 1, 2, 1, 16, 8000, [1, 333]),
+    (2, 2, 3, 3, 16, 48, [2, 40]),
+    (3, 17, 4, 2, 32, 64, [17, 20, 90]),
+    (2, 64, 2, 1, 64, 128, [64, 200]),
+    (2, 150, 3, 3, 16, 208, [150, 170]),
+    (1, 257, 2, 2, 128, 0, [300]),
+    (1, 130, 2, 2, 32, 0, [130]),
+]
+
+
+@pytest.mark.parametrize("n_seq,T,H,G,page,n_shared,tails", CASES)
+def test_attention_against_64_bits(cuda, n_seq, T, H, G, page, n_shared, tails):
+    n_new = [T if t >= T else max(t, 0) for t in tails]
+    n_new = [min(n, T - b % 3) if T > 3 else n for b, n in enumerate(n_new)]  # a padded batch
+    uniform = T == 1 and all(t >= 1 for t in tails)
+    if T == 1 and not uniform:
+        n_new = [1 if t >= 0 else 0 for t in tails]
+    c, Q, shared, want = build(cuda, n_seq, T, H, G, page, n_shared, tails, n_new, n_seq + T)
+    out = torch.full((n_seq * T, H * 64), 7.0, dtype=torch.bfloat16, device=cuda)
+    ops.attention_pages(Q, c, 1, H, T=T, n_new=None if uniform else i32(n_new),
+                        max_ctx=n_shared + max(tails + [1]), shared_pages=shared,
+                        n_shared=n_shared, out=out)
+    check(out, want, T, H, n_new)
+    # the prefix read through each table row, and the loosest bound on the lengths
+    if n_shared:
+        again = torch.full_like(out, 7.0)
+        ops.attention_pages(Q, c, 1, H, T=T, n_new=i32(n_new), out=again)
+        check(again, want, T, H, n_new)
+
+
+def test_a_sequence_that_ends_inside_the_prefix(cuda):
+    """n_ctx below n_shared: the row sees its own n_ctx keys of the prefix only; with
+    none, or more new rows than positions, rows are zero."""
+    c, Q, shared, _ = build(cuda, 4, 3, 2, 2, 16, 160, [3, 3, 3, 3], [3] * 4, 3, junk=0.0)
+    lens = [163, 50, 2, 0]
+    c.n_ctx.copy_(i32(lens))
+    out = ops.attention_pages(Q, c, 1, 2, T=3, max_ctx=163, shared_pages=shared, n_shared=160)
+    k64, v64 = c.K[:, 1].double().cpu().numpy(), c.V[:, 1].double().cpu().numpy()
+    table = c.table.cpu().numpy()
+    want = []
+    for b, n in enumerate(lens):
+        kb = k64[table[b]].transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:n]
+        vb = v64[table[b]].transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:n]
+        want.append(po.attention(Q.double().cpu().numpy().reshape(4, 3, 2, 64)[b], kb, vb, 3))
+    check(out, want, 3, 2, [3] * 4)
+    assert (want[3][0] == 0).all() and (want[2][0][0] == 0).all()
+
+
+@pytest.mark.parametrize("n_seq,T", [(3, 1), (40, 1), (2, 70)])
+def test_keys_nobody_sees_may_hold_anything(cuda, n_seq, T):
+    """NaN, infinities and the lowest finite value in rows behind the sequences give
+    the bits that zeros there give."""
+    outs = []
+    for junk in (0.0, float("nan"), float("inf"), -float("inf"), torch.finfo(torch.bfloat16).min):
+        tails = [T + 3 * i for i in range(n_seq)]
+        c, Q, shared, _ = build(cuda, n_seq, T, 4, 2, 32, 96, tails, [T] * n_seq, 5, junk=junk)
+        outs.append(ops.attention_pages(Q, c, 1, 4, T=T, max_ctx=96 + max(tails),
+                                        shared_pages=shared, n_shared=96))
+    for o in outs[1:]:
+        assert torch.equal(outs[0].view(torch.int16), o.view(torch.int16))
+
+
+@pytest.mark.parametrize("n_seq,T,n_shared", [(2, 1, 512), (64, 1, 512), (2, 130, 512), (3, 1, 0)])
+def test_large_scores(cuda, n_seq, T, n_shared):
+    """Scores of some hundreds, growing along the keys and falling: the running
+    maximum moves all the way. The 32-bit scores are off by 2^-24 of sums of 64
+    products of up to 2^9 each; exponentials by that of a score in absolute terms,
+    64 * 2^9 / 8 * 2^-24 = 2^-12 of the weight."""
+    for sign in (1.0, -1.0):
+        tails = [T + 40] * n_seq
+        c, Q, shared, _ = build(cuda, n_seq, T, 2, 2, 16, n_shared, tails, [T] * n_seq, 9, scale=0)
+        n = n_shared + T + 40
+        Q.fill_(4.0)
+        table = c.table.cpu().numpy()
+        ramp = torch.linspace(-8, 8, n, device=cuda) * sign
+        for b in range(n_seq):
+            for k in range(table.shape[1]):
+                if table[b, k] < 0:
+                    continue
+                rows = min(16, n - 16 * k)
+                c.K[table[b, k], :, :, :rows] = ramp[16 * k:16 * k + rows, None].bfloat16()
+        out = ops.attention_pages(Q, c, 1, 2, T=T, max_ctx=n, shared_pages=shared,
+                                  n_shared=n_shared)
+        k64, v64 = c.K[:, 1].double().cpu().numpy(), c.V[:, 1].double().cpu().numpy()
+        want = []
+        for b in range(n_seq):
+            p = table[b, :-(-n // 16)]
+            kb = k64[p].transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:n]
+            vb = v64[p].transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:n]
+            want.append(po.attention(np.full((T, 2, 64), 4.0), kb, vb, T))
+        check(out, want, T, 2, [T] * n_seq)
+
+
+def test_bad_entries_read_as_zeros_and_are_recorded(cuda):
+    for bad in (-5, 10 ** 6):
+        c, Q, shared, _ = build(cuda, 3, 1, 2, 2, 16, 32, [40, 40, 40], [1] * 3, 2, junk=0.0)
+        good = ops.attention_pages(Q, c, 1, 2, max_ctx=72, shared_pages=shared, n_shared=32)
+        assert ops.device_error() == 0
+        p = int(c.table[1, 3])
+        c.table[1, 3] = bad
+        got = ops.attention_pages(Q, c, 1, 2, max_ctx=72, shared_pages=shared, n_shared=32)
+        assert ops.device_error() == 0x1601
+        assert torch.equal(got[[0, 2]], good[[0, 2]])
+        c.table[1, 3] = p
+        c.K[p] = 0
+        c.V[p] = 0
+        want = ops.attention_pages(Q, c, 1, 2, max_ctx=72, shared_pages=shared, n_shared=32)
+        assert torch.equal(got, want)
+
+
+def test_a_pool_behind_32_bit_offsets(cuda):
+    """Pages more than 2^32 elements into the pools."""
+    n_pages, L, G, page = 1100, 64, 16, 64  # 4.6e9 elements a pool, 9.2 GB
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    K = torch.empty(n_pages, L, G, page, 64, dtype=torch.bfloat16, device=cuda)
+    V = torch.empty_like(K)
+    c = PageCache(K, V, i32([[n_pages - 1, n_pages - 3], [n_pages - 2, -1]]), i32([100, 0]),
+                  i32([0] * (n_pages - 3) + [1, 0, 1]))
+    assert (n_pages - 3) * K.stride(0) > 2 ** 32
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(100, G * 64, generator=g, device=cuda).bfloat16()
+    y = torch.randn(100, G * 64, generator=g, device=cuda).bfloat16()
+    for layer in (0, L - 1):
+        ops.pages_write(c, layer, x, y, i32([0]), T=100)
+        assert torch.equal(K[n_pages - 1, layer].transpose(0, 1).reshape(64, -1), x[:64])
+        assert torch.equal(V[n_pages - 3, layer, :, :36].transpose(0, 1).reshape(36, -1), y[64:])
+    c.table[1, 0] = -1
+    c.refs[:n_pages - 3] = 1
+    assert ops.pages_fork(c, i32([0]), i32([1])).item() == 0
+    assert c.table[1].tolist() == [n_pages - 1, n_pages - 2]
+    assert torch.equal(V[n_pages - 2, L - 1, :, :36], V[n_pages - 3, L - 1, :, :36])
+    Q = torch.randn(2, G * 64, generator=g, device=cuda).bfloat16()
+    out = ops.attention_pages(Q, c, L - 1, G, max_ctx=100)
+    q = Q.double().cpu().numpy().reshape(2, 1, G, 64)
+    want = [po.attention(q[b], *(t.double().cpu().numpy().reshape(100, G, 64) for t in (x, y)), 1)
+            for b in range(2)]
+    check(out, want, 1, G, [1, 1])
+    ops.pages_copy(K, V, i32([n_pages - 1]), K, V, i32([n_pages - 4]))
+    assert torch.equal(K[n_pages - 4].view(torch.int16), K[n_pages - 1].view(torch.int16))
+    # the pages at the end go to the front
+    c.refs[:n_pages - 3] = 0
+    assert ops.pages_compact(c).item() == 3
+    assert c.table.tolist() == [[2, 0], [2, 1]]
+    assert torch.equal(ops.attention_pages(Q, c, L - 1, G, max_ctx=100), out)
+
+
+# ---- streams, graphs, refusals -----------------------------------------------
+
+def test_another_stream_and_captured_graphs(cuda):
+    """A decode step (extend, write, attend) captured once and replayed as the
+    sequences grow over page ends gives what the eager steps give."""
+    def steps(replay):
+        c, _ = make(cuda, 40, 4, 6, n_layer=1, n_kv=2, page=16, seed=4)
+        ops.pages_extend(c, i32([32, 0, 0, 0]))
+        ops.pages_fork(c, i32([0, 0, 0]), i32([1, 2, 3]))
+        x = torch.zeros(4, 128, dtype=torch.bfloat16, device=cuda)
+        one, out = i32([1, 1, 1, 1]), torch.zeros(4, 256, dtype=torch.bfloat16, device=cuda)
+        q = torch.zeros(4, 256, dtype=torch.bfloat16, device=cuda)
+        shared = c.table[0, :2].clone()
+
+        def step():
+            pos0 = ops.pages_extend(c, one)
+            ops.pages_write(c, 0, x, x, pos0)
+            ops.attention_pages(q, c, 0, 4, max_ctx=96, shared_pages=shared, n_shared=32, out=out)
+
+        graph = None
+        got = []
+        g = torch.Generator(device=cuda).manual_seed(8)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for i in range(40):
+                x.copy_(torch.randn(4, 128, generator=g, device=cuda))
+                q.copy_(torch.randn(4, 256, generator=g, device=cuda))
+                if not replay or i == 0:
+                    step()
+                else:
+                    if graph is None:
+                        graph = torch.cuda.CUDAGraph()
+                        with torch.cuda.graph(graph, stream=s):
+                            step()
+                    graph.replay()
+                got.append(out.clone())
+        s.synchronize()
+        assert c.n_ctx.tolist() == [72] * 4
+        return torch.stack(got), c
+    a, ca = steps(False)
+    b, cb = steps(True)
+    assert torch.equal(a, b) and torch.equal(ca.table, cb.table)
+    assert torch.equal(ca.refs, cb.refs)
+    assert ca.refs.sum().item() == 4 * 5 and ca.table[:, :2].unique().numel() == 2
+
+
+def test_front_end_refusals(cuda):
+    c, _ = make(cuda, 8, 2, 4)
+    f = dict(device=cuda)
+    Q = torch.zeros(2, 192, dtype=torch.bfloat16, **f)
+    one = i32([0, 1])
+    with pytest.raises(TypeError):
+        ops.pages_extend(c, torch.ones(2, **f))
+    with pytest.raises(ValueError):
+        ops.pages_extend(c, i32([1, 1, 1]))
+    with pytest.raises(ValueError):
+        ops.pages_extend(c, torch.ones(2, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops.pages_fork(c, one, i32([1]))
+    with pytest.raises(ValueError):
+        ops.pages_free(c, i32([0, 1, 0, 1])[::2])
+    with pytest.raises(ValueError):
+        ops.pages_write(c, 0, Q, Q, i32([0]))            # two rows, one sequence
+    with pytest.raises(ValueError):
+        ops.attention_pages(Q, c, 0, 3, n_shared=16, shared_pages=i32([]))
+    with pytest.raises(ValueError):
+        ops.attention_pages(Q, c, 0, 3, n_shared=16)
+    with pytest.raises(TypeError):
+        ops.attention_pages(Q.float(), c, 0, 3)
+    ws = torch.empty(8, dtype=torch.uint8, **f)
+    bad = [dict(layer=2), dict(layer=-1), dict(n_head=4, Q=torch.zeros(2, 256, dtype=torch.bfloat16, **f)),
+           dict(max_ctx=0), dict(n_shared=8, shared_pages=one), dict(workspace=ws, max_ctx=64),
+           dict(n_shared=32, max_ctx=16, shared_pages=one),
+           dict(Q=torch.zeros(3, 192, dtype=torch.bfloat16, **f))]
+    for kw in bad:
+        kw = dict(dict(Q=Q, layer=0, n_head=3), **kw)
+        with pytest.raises(_lib.W8A8Error) as e:
+            ops.attention_pages(kw.pop("Q"), c, kw.pop("layer"), kw.pop("n_head"), **kw)
+        assert e.value.status == _lib.W8A8_ERR_INVALID, kw
+    with pytest.raises(_lib.W8A8Error):
+        ops.pages_write(c, 5, Q, Q, one)
+    with pytest.raises(_lib.W8A8Error):
+        ops.pages_write(c, 0, Q.view(-1)[4:4 + 192].view(1, 192), Q[:1], i32([0]))
+    with pytest.raises(_lib.W8A8Error):
+        ops.pages_compact(c, workspace=ws)
+    assert c.n_ctx.tolist() == [0, 0]
+
+
+def test_the_slot_cache_attention_agrees(cuda):
+    """The framework's path over both caches: the packed QKV projection writes new
+    rows into the slot cache and, through pages_write, into pages; decode attention
+    over the two differs by the roundings of the slot cache's kernel (scores rounded
+    to bf16, 2^-8 of |s| <= 8, in the weights, and its own rounded weights)."""
+    d, H, n = 768, 12, 100
+    g = torch.Generator(device=cuda).manual_seed(0)
+    X = torch.randn(4 * n, d, generator=g, device=cuda).bfloat16()
+    W = torch.randint(-127, 128, (3 * d, d), generator=g, device=cuda, dtype=torch.int8)
+    sW = torch.full((3 * d,), 5e-4, device=cuda)
+    bias = torch.zeros(3 * d, device=cuda).bfloat16()
+    Xq, sX = ops.per_token_quant(X)
+    Q = torch.empty(4 * n, d, dtype=torch.bfloat16, device=cuda)
+    Kc = torch.empty(4, n, d, dtype=torch.bfloat16, device=cuda)
+    Vc = torch.empty_like(Kc)
+    ops.linear_qkv(Xq, sX, W, sW, bias, Q, Kc, Vc, n * d, n)
+    c = PageCache.empty(40, 4, 8, 1, H, 16, cuda)
+    pos0 = ops.pages_extend(c, i32([n] * 4))
+    ops.pages_write(c, 0, Kc.view(4 * n, d), Vc.view(4 * n, d), pos0, T=n)
+    q = Q.view(4, n, d)[:, -1].contiguous()
+    slot = ops.attention_decode(q, Kc, Vc, n * d, i32([n] * 4), n, H)
+    page = ops.attention_pages(q, c, 0, H)
+    k64, v64 = (t.double().cpu().numpy().reshape(4, n, H, 64) for t in (Kc, Vc))
+    q64 = q.double().cpu().numpy().reshape(4, 1, H, 64)
+    want = [po.attention(q64[b], k64[b], v64[b], 1) for b in range(4)]
+    check(page, want, 1, H, [1] * 4)
+    smax = max(np.abs(np.einsum("nhd,hd->nh", k64[b], q64[b, 0])).max() / 8 for b in range(4))
+    A = np.stack([w[1][0] for w in want]).reshape(4, d)
+    err = (slot.double() - page.double()).abs().cpu().numpy()
+    assert (err <= (2.0 ** -8 * (2 * smax + 6)) * A).all()
