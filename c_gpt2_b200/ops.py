@@ -16,7 +16,8 @@ from ._lib import check, core
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the stream's handle without building a torch.cuda.Stream (0.3 against 3.2 us a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -331,48 +332,63 @@ def attention_decode_quant(Q, Kc, Vc, seq_stride, n_ctx, max_ctx, n_head, worksp
 
 
 # ---- cache pages (c_gpt2_b200/pages.py) ----
+# A decode step makes these calls for every token, and its kernels take a few
+# microseconds: the checks are written to cost little.
 
-def _here(t: torch.Tensor | None, dtype: torch.dtype, name: str, shape: tuple | None = None) -> int | None:
-    """Address of a contiguous tensor of this dtype (and shape) on the current device."""
-    if t is None:
-        return None
+_I32, _BF16, _U8 = torch.int32, torch.bfloat16, torch.uint8
+
+
+def _here(t: torch.Tensor, dtype: torch.dtype, dev: int, name: str, n: int | None = None) -> int:
+    """Address of a contiguous tensor of this dtype on device `dev`, of n values in
+    one dimension unless n is None."""
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: expected a tensor on the current CUDA device")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: expected a tensor on the cache's CUDA device")
     if not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if n is not None and t.shape != (n,):
+        raise ValueError(f"{name}: expected shape ({n},), got {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
-    """Address of bf16 rows [rows, cols] (row-strided) on the current device."""
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{name}: expected {torch.bfloat16}, got {t.dtype}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: expected a tensor on the current CUDA device")
-    if tuple(t.shape) != (rows, cols) or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: expected [{rows}, {cols}] with contiguous rows")
-    return t.data_ptr()
+def _rows(t: torch.Tensor, rows: int, cols: int, dev: int, name: str) -> tuple[int, int]:
+    """Address and row stride of bf16 rows [rows, cols] on device `dev`."""
+    if t.dtype != _BF16:
+        raise TypeError(f"{name}: expected {_BF16}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: expected a tensor on the cache's CUDA device")
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name}: expected [{rows}, {cols}], got {tuple(t.shape)}")
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"{name}: expected contiguous rows")
+    return t.data_ptr(), ld if rows > 1 else cols
 
 
-def _cache(cache):
-    if cache.device.type != "cuda" or cache.device.index != torch.cuda.current_device():
-        raise ValueError("cache: expected a cache on the current CUDA device")
-    return cache._ref
+def _device_of(cache) -> int:
+    return _current(cache.index, "cache")
+
+
+def _current(dev: int, name: str) -> int:
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected tensors on the current CUDA device")
+    return dev
+
+
+def _raw_stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def pages_extend(cache, n_new, pos0=None):
     """Room for n_new[s] more positions of every slot s (int32 [n_slot]). Returns
     pos0 [n_slot]: the first new position, -1 where none were asked for, -2 where
     the pages did not suffice and the slot was left as it was."""
-    c = _cache(cache)
+    dev = _device_of(cache)
     pos0 = pos0 if pos0 is not None else torch.empty_like(cache.n_ctx)
-    shape = (cache.n_slot,)
-    check(core().w8a8_pages_extend(c, _here(n_new, torch.int32, "n_new", shape),
-                                   _here(pos0, torch.int32, "pos0", shape), _stream()),
+    n = cache.n_slot
+    check(core().w8a8_pages_extend(cache.ref, _here(n_new, _I32, dev, "n_new", n),
+                                   _here(pos0, _I32, dev, "pos0", n), _raw_stream(dev)),
           "w8a8_pages_extend")
     return pos0
 
@@ -380,75 +396,87 @@ def pages_extend(cache, n_new, pos0=None):
 def pages_write(cache, layer, K, V, pos0, T=1, n_new=None):
     """Rows b*T + t of K, V [n_seq*T, n_kv_head*64] become position pos0[b] + t of
     slot b's pages of this layer, for t < n_new[b] (default: all T), pos0[b] >= 0."""
-    c = _cache(cache)
+    dev = _device_of(cache)
     n_seq, d = pos0.numel(), cache.n_kv_head * 64
-    shape = (n_seq,)
-    check(core().w8a8_pages_write(c, layer, _rows(K, n_seq * T, d, "K"), K.stride(0),
-                                  _rows(V, n_seq * T, d, "V"), V.stride(0), n_seq, T,
-                                  _here(n_new, torch.int32, "n_new", shape),
-                                  _here(pos0, torch.int32, "pos0", shape), _stream()),
-          "w8a8_pages_write")
+    k, ldk = _rows(K, n_seq * T, d, dev, "K")
+    v, ldv = _rows(V, n_seq * T, d, dev, "V")
+    check(core().w8a8_pages_write(
+        cache.ref, layer, k, ldk, v, ldv, n_seq, T,
+        None if n_new is None else _here(n_new, _I32, dev, "n_new", n_seq),
+        _here(pos0, _I32, dev, "pos0", n_seq), _raw_stream(dev)), "w8a8_pages_write")
 
 
 def pages_fork(cache, src, dst, status=None):
     """Slot dst[i] (empty) goes on from slot src[i]. Returns status [n]: 0, or 1
     where the entry named no such slots, one not empty or one named before, or 2
     where no page was left; those entries did nothing."""
-    c = _cache(cache)
+    dev = _device_of(cache)
     status = status if status is not None else torch.empty_like(src)
-    shape = (src.numel(),)
-    check(core().w8a8_pages_fork(c, _here(src, torch.int32, "src", shape),
-                                 _here(dst, torch.int32, "dst", shape), shape[0],
-                                 _here(status, torch.int32, "status", shape), _stream()),
+    n = src.numel()
+    check(core().w8a8_pages_fork(cache.ref, _here(src, _I32, dev, "src", n),
+                                 _here(dst, _I32, dev, "dst", n), n,
+                                 _here(status, _I32, dev, "status", n), _raw_stream(dev)),
           "w8a8_pages_fork")
     return status
 
 
 def pages_free(cache, slots):
     """The slots (int32, device) give their pages back and are empty."""
-    c = _cache(cache)
-    check(core().w8a8_pages_free(c, _here(slots, torch.int32, "slots"), slots.numel(), _stream()),
-          "w8a8_pages_free")
+    dev = _device_of(cache)
+    check(core().w8a8_pages_free(cache.ref, _here(slots, _I32, dev, "slots"), slots.numel(),
+                                 _raw_stream(dev)), "w8a8_pages_free")
 
 
 def pages_compact(cache, n_live=None, workspace=None):
     """Moves the pages in use to the front of the pool; returns their number (int32
     [1], device)."""
-    c = _cache(cache)
-    n_live = n_live if n_live is not None else torch.empty(1, dtype=torch.int32,
-                                                           device=cache.device)
+    dev = _device_of(cache)
+    n_live = n_live if n_live is not None else cache.n_ctx.new_empty(1)
     if workspace is None:
         workspace = torch.empty(core().w8a8_pages_compact_workspace_size(cache.n_pages),
-                                dtype=torch.uint8, device=cache.device)
-    check(core().w8a8_pages_compact(c, _here(n_live, torch.int32, "n_live", (1,)),
-                                    _here(workspace, torch.uint8, "workspace"),
-                                    workspace.numel(), _stream()), "w8a8_pages_compact")
+                                dtype=_U8, device=cache.device)
+    check(core().w8a8_pages_compact(cache.ref, _here(n_live, _I32, dev, "n_live", 1),
+                                    _here(workspace, _U8, dev, "workspace"), workspace.numel(),
+                                    _raw_stream(dev)), "w8a8_pages_compact")
     return n_live
+
+
+def _pool(t: torch.Tensor, like: torch.Tensor, dev: int, name: str) -> int:
+    """Address of a bf16 pool of contiguous pages shaped and strided as `like`."""
+    if t.dtype != _BF16:
+        raise TypeError(f"{name}: expected {_BF16}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device")
+    if t is not like and (t.shape != like.shape or t.stride() != like.stride()):
+        raise ValueError(f"{name}: expected shape and strides of its pair")
+    return t.data_ptr()
+
+
+def _page_size(t: torch.Tensor, name: str) -> tuple[tuple, int, int]:
+    """Shape of a pool's pages, their elements, and the pool's page stride."""
+    shape, strides = t.shape, t.stride()
+    size = 1
+    for n, s in zip(reversed(shape[1:]), reversed(strides[1:])):
+        if n != 1 and s != size:
+            raise ValueError(f"{name}: expected contiguous pages")
+        size *= n
+    return shape[1:], size, strides[0] if shape[0] > 1 else size
 
 
 def pages_copy(Ksrc, Vsrc, src, Kdst, Vdst, dst):
     """Pages src[i] of the pools Ksrc, Vsrc to pages dst[i] of Kdst, Vdst (the first
     dimension counts pages). The dst pages are distinct, and none is a source."""
+    dev = _current(Ksrc.get_device(), "Ksrc")
     n = src.numel()
-    size = Ksrc[0].numel()
-    for name, t in (("Ksrc", Ksrc), ("Vsrc", Vsrc), ("Kdst", Kdst), ("Vdst", Vdst)):
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"{name}: expected {torch.bfloat16}, got {t.dtype}")
-        if not t.is_cuda or t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name}: expected a tensor on the current CUDA device")
-        if t.shape[1:] != Ksrc.shape[1:] or not t[0].is_contiguous():
-            raise ValueError(f"{name}: expected contiguous pages of {tuple(Ksrc.shape[1:])}")
-    if Ksrc.shape != Vsrc.shape or Ksrc.stride() != Vsrc.stride():
-        raise ValueError("Ksrc, Vsrc: expected the same shape and strides")
-    if Kdst.shape != Vdst.shape or Kdst.stride() != Vdst.stride():
-        raise ValueError("Kdst, Vdst: expected the same shape and strides")
-    ss = Ksrc.stride(0) if Ksrc.shape[0] > 1 else size
-    ds = Kdst.stride(0) if Kdst.shape[0] > 1 else size
-    check(core().w8a8_pages_copy(Ksrc.data_ptr(), Vsrc.data_ptr(), ss, Ksrc.shape[0],
-                                 Kdst.data_ptr(), Vdst.data_ptr(), ds, Kdst.shape[0], size,
-                                 _here(src, torch.int32, "src", (n,)),
-                                 _here(dst, torch.int32, "dst", (n,)), n, _stream()),
-          "w8a8_pages_copy")
+    page, size, ss = _page_size(Ksrc, "Ksrc")
+    page_dst, _, ds = _page_size(Kdst, "Kdst")
+    if page != page_dst:
+        raise ValueError(f"Kdst: expected pages of {tuple(page)}, got {tuple(page_dst)}")
+    check(core().w8a8_pages_copy(
+        _pool(Ksrc, Ksrc, dev, "Ksrc"), _pool(Vsrc, Ksrc, dev, "Vsrc"), ss, Ksrc.shape[0],
+        _pool(Kdst, Kdst, dev, "Kdst"), _pool(Vdst, Kdst, dev, "Vdst"), ds, Kdst.shape[0], size,
+        _here(src, _I32, dev, "src", n), _here(dst, _I32, dev, "dst", n), n, _raw_stream(dev)),
+        "w8a8_pages_copy")
 
 
 def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shared_pages=None,
@@ -458,26 +486,26 @@ def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shar
     rows of the output are left as they were). The first n_shared positions are
     read, once for the batch, from shared_pages (int32, device); max_ctx (default:
     the table's) bounds every length."""
-    c = _cache(cache)
+    dev = _device_of(cache)
     d = n_head * 64
     n_seq = Q.shape[0] // T if T > 0 else 0
     if max_ctx is None:
         max_ctx = cache.max_pages * cache.page
     if n_shared > 0 and (shared_pages is None or shared_pages.numel() * cache.page < n_shared):
         raise ValueError("shared_pages: expected a page for every n_shared position")
-    q = _rows(Q, n_seq * T, d, "Q")
-    O = out if out is not None else torch.empty((n_seq * T, d), dtype=torch.bfloat16,
-                                                device=Q.device)
+    q, ldq = _rows(Q, n_seq * T, d, dev, "Q")
+    O = out if out is not None else Q.new_empty((n_seq * T, d))
+    o, ldo = _rows(O, n_seq * T, d, dev, "out")
     if workspace is None:
         need = core().w8a8_attention_pages_workspace_size(n_seq, T, n_head, cache.n_kv_head,
                                                           max_ctx, n_shared)
-        workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
-    check(core().w8a8_attention_pages(c, layer, q, Q.stride(0), n_seq, T,
-                                      _here(n_new, torch.int32, "n_new", (n_seq,)), max_ctx,
-                                      _here(shared_pages, torch.int32, "shared_pages"), n_shared,
-                                      n_head, 64, _rows(O, n_seq * T, d, "out"), O.stride(0),
-                                      _here(workspace, torch.uint8, "workspace"),
-                                      workspace.numel(), _stream()), "w8a8_attention_pages")
+        workspace = torch.empty(need, dtype=_U8, device=cache.device)
+    check(core().w8a8_attention_pages(
+        cache.ref, layer, q, ldq, n_seq, T,
+        None if n_new is None else _here(n_new, _I32, dev, "n_new", n_seq), max_ctx,
+        None if shared_pages is None else _here(shared_pages, _I32, dev, "shared_pages"),
+        n_shared, n_head, 64, o, ldo, _here(workspace, _U8, dev, "workspace"),
+        workspace.numel(), _raw_stream(dev)), "w8a8_attention_pages")
     return O
 
 

@@ -25,7 +25,7 @@ class PageCache:
     table [n_slot, max_pages], n_ctx [n_slot], refs [n_pages] int32."""
 
     __slots__ = ("K", "V", "table", "n_ctx", "refs", "device", "n_pages", "n_layer", "n_kv_head",
-                 "page", "n_slot", "max_pages", "_c", "_ref")
+                 "page", "n_slot", "max_pages", "index", "c", "ref")
 
     def __init__(self, K: torch.Tensor, V: torch.Tensor, table: torch.Tensor,
                  n_ctx: torch.Tensor, refs: torch.Tensor):
@@ -48,12 +48,13 @@ class PageCache:
             raise ValueError("the cache's tensors are on different devices")
         self.n_slot, self.max_pages = table.shape
         self.device = K.device
+        self.index = K.get_device()  # -1: not on a GPU
         self.K, self.V, self.table, self.n_ctx, self.refs = K, V, table, n_ctx, refs
-        self._c = _lib.Pages(K.data_ptr(), V.data_ptr(),
-                             K.stride(0) if self.n_pages > 1 else K[0].numel(), self.n_pages,
-                             self.page, self.n_layer, self.n_kv_head, table.data_ptr(),
-                             self.max_pages, self.n_slot, n_ctx.data_ptr(), refs.data_ptr())
-        self._ref = ctypes.byref(self._c)
+        self.c = _lib.Pages(K.data_ptr(), V.data_ptr(),
+                            K.stride(0) if self.n_pages > 1 else K[0].numel(), self.n_pages,
+                            self.page, self.n_layer, self.n_kv_head, table.data_ptr(),
+                            self.max_pages, self.n_slot, n_ctx.data_ptr(), refs.data_ptr())
+        self.ref = ctypes.byref(self.c)  # w8a8_pages *
 
     @classmethod
     def empty(cls, n_pages: int, n_slot: int, max_pages: int, n_layer: int, n_kv_head: int,

@@ -114,9 +114,9 @@ def test_page_cache_takes_one_page_and_strided_pages():
     one = _cpu_cache(K=torch.zeros(1, 2, 3, 16, 64, dtype=torch.bfloat16),
                      V=torch.zeros(1, 2, 3, 16, 64, dtype=torch.bfloat16),
                      refs=torch.zeros(1, dtype=torch.int32))
-    assert one._c.page_stride == 2 * 3 * 16 * 64
+    assert one.c.page_stride == 2 * 3 * 16 * 64
     kv = torch.zeros(8, 2, 2, 3, 16, 64, dtype=torch.bfloat16)  # K and V of a page side by side
-    assert _cpu_cache(K=kv[:, 0], V=kv[:, 1])._c.page_stride == 2 * 2 * 3 * 16 * 64
+    assert _cpu_cache(K=kv[:, 0], V=kv[:, 1]).c.page_stride == 2 * 2 * 3 * 16 * 64
 
 
 # ---- the oracle itself ------------------------------------------------------
