@@ -145,7 +145,7 @@ __device__ __forceinline__ Row get_row(const ApArgs &a, int seq, int kvh, int64_
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -448,7 +448,7 @@ constexpr int kTcKeys = 128;
 constexpr int kTcStages = 5;
 constexpr uint32_t kTcTile = kTcKeys * 128;  // Q tile, or K or V of a block: 16 KB
 constexpr int kTcTmaWarp = 8, kTcMmaWarp = 9;
-constexpr int kTcThreads = 10 * 32;
+constexpr int kTcThreads = 12 * 32;  // three warpgroups; the last two warps only pass registers
 constexpr int kTcSoftThreads = 8 * 32;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 192, kColGroup = 256;
 constexpr float kMaxSlack = 8.0f;  // base 2
@@ -458,9 +458,11 @@ struct TcCtl {
   uint64_t q_full;
   uint64_t kv_full[kTcStages], kv_empty[kTcStages];
   uint64_t s_full[2], s_free[2], p_full[2], o_done[2];
-  uint64_t drain;
+  uint64_t turn[2][4];  // group g's, of a quarter
+  uint64_t v_ready, drain;
   uint32_t tmem_base;
   int abort_flag;
+  int idle[8];
   float2 ml[kTileRows];  // group 1's, where both groups work on one tile
 };
 
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t *sQ = smem;                       // [2] tiles
   uint8_t *sKV = smem + 2 * kTcTile;        // [stages] K, V
   TcCtl *ctl = reinterpret_cast<TcCtl *>(sKV + kTcStages * 2 * kTcTile);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
   pdl_wait();
   const TcItem it = get_tc_item(a, blockIdx.x);
@@ -535,6 +537,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (n_rows <= 0 || (blocks == 0 && !a.direct)) return;
   const bool one = n_rows <= kTileRows;      // both groups on one tile
   const int units = one ? blocks : 2 * blocks;  // unit u: group u & 1
+  // the last block reaches behind the positions that hold anything
+  const bool v_cut = it.k0 + blocks * kTcKeys > it.n_valid;
   if (threadIdx.x == 0) {
     mbar_init(&ctl->q_full, 8);
     for (int i = 0; i < kTcStages; ++i) {
@@ -547,6 +551,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&ctl->p_full[i], 4);
       mbar_init(&ctl->o_done[i], 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&ctl->turn[i >> 2][i & 3], 1);
+    mbar_init(&ctl->v_ready, 1);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_barrier_init();
@@ -563,113 +569,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = ctl->tmem_base;
   volatile int *abort_flag = &ctl->abort_flag;
 
-  if (warp == kTcTmaWarp) {
-    // ---------------- TMA: lane i < 2 * boxes issues one box of a block ----------------
-    const int box = min(1 << a.page_shift, kStageKeys);  // rows
-    const int boxes = kTcKeys / box;
-    const bool act = lane < 2 * boxes;
-    const bool is_v = lane >= boxes;
-    const int bx = is_v ? lane - boxes : lane;
-    auto entry = [&](int j) -> int {  // page of this lane's box, n_pages: reads as zeros
-      const int pos = it.k0 + j * kTcKeys + bx * box;
-      if (!act || pos >= it.k1) return a.n_pages;
-      const int k = pos >> a.page_shift;
-      int p = -1;
-      if (pos < a.n_shared) p = a.shared[k];
-      else if (k < a.max_pages) p = a.table[(int64_t)it.b * a.max_pages + k];
-      if (p < 0 || p >= a.n_pages) {
-        report_error(a.err, kErrEntry);
-        p = a.n_pages;
-      }
-      return p;
-    };
-    int p = blocks ? entry(0) : 0;
-    int n = 0;
-    for (; n < blocks; ++n) {
-      const int next = n + 1 < blocks ? entry(n + 1) : 0;
-      const int st = n % kTcStages;
-      bool ok = true;
-      if (n >= kTcStages)
-        ok = mbar_wait(&ctl->kv_empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag, a.err, kErrTc);
-      if (!__all_sync(~0u, ok)) break;
-      if (lane == 0) mbar_arrive_expect_tx(&ctl->kv_full[st], 2 * kTcTile);
-      __syncwarp();
-      if (act) {
-        const int pos = it.k0 + n * kTcKeys + bx * box;
-        const int y = (it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-        tma_load_3d(sKV + (st * 2 + is_v) * kTcTile + bx * box * 128, is_v ? &tmV : &tmK,
-                    &ctl->kv_full[st], 0, y, p);
-      }
-      p = next;
-    }
-    if (*abort_flag)  // no copy may still be writing shared memory when the CTA exits
-      for (int i = n > kTcStages ? n - kTcStages : 0; i < n; ++i)
-        mbar_wait(&ctl->kv_full[i % kTcStages], (i / kTcStages) & 1, nullptr, a.err, kErrTc + 1);
-  } else if (warp == kTcMmaWarp) {
-    // ---------------- MMA ----------------
-    const uint32_t idS = make_idesc(1, 1, kTileRows, kTcKeys);
-    const uint32_t idO = make_idesc_bmn(1, 1, kTileRows, kPageHd);
-    const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
-    bool ok = mbar_wait(&ctl->q_full, 0, abort_flag, a.err, kErrTc + 2);
-    int seen = 0;  // blocks known to be in shared memory
-    auto issue_s = [&](int u) -> bool {
-      const int g = u & 1, i = u >> 1, j = one ? u : i;  // group, its unit, block
-      if (i > 0 && !mbar_wait(&ctl->s_free[g], (i - 1) & 1, abort_flag, a.err, kErrTc + 3))
-        return false;
-      const int st = j % kTcStages;
-      if (j >= seen) {
-        if (!mbar_wait(&ctl->kv_full[st], (j / kTcStages) & 1, abort_flag, a.err, kErrTc + 4))
-          return false;
-        seen = j + 1;
-        const int first = it.n_valid - (it.k0 + j * kTcKeys);
-        if (first < kTcKeys) {
-          // rows of the last page that hold nothing yet: 0 * V must stay 0
-          uint8_t *v = sKV + (st * 2 + 1) * kTcTile;
-          for (int x = max(first, 0) * 8 + lane; x < kTcKeys * 8; x += 32)
-            *reinterpret_cast<uint4 *>(v + x * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t qa = q_addr + (one ? 0 : g) * kTcTile, ka = kv_addr + st * 2 * kTcTile;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc_mma_bf16(tmem + g * kColGroup + kColS, make_sw128_desc(qa + 32 * k),
-                      make_sw128_desc(ka + 32 * k), idS, k > 0);
-        tc_commit(&ctl->s_full[g]);
-      }
-      __syncwarp();
-      return true;
-    };
-    auto issue_o = [&](int u) -> bool {
-      const int g = u & 1, i = u >> 1, j = one ? u : i;
-      if (!mbar_wait(&ctl->p_full[g], i & 1, abort_flag, a.err, kErrTc + 5)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t base = tmem + g * kColGroup;
-        const uint32_t va = kv_addr + (j % kTcStages * 2 + 1) * kTcTile;
-#pragma unroll
-        for (int k = 0; k < kTcKeys / 16; ++k)
-          tc_mma_bf16_ta(base + kColO, base + kColP + 8 * k, make_sw128_mn_desc(va + k * 2048),
-                         idO, i > 0 || k > 0);
-        tc_commit(&ctl->o_done[g]);
-        if (one || g == 1) tc_commit(&ctl->kv_empty[j % kTcStages]);
-      }
-      __syncwarp();
-      return true;
-    };
-    for (int u = 0; u < 2 && u < units && ok; ++u) ok = issue_s(u);
-    for (int u = 0; u < units && ok; u += 2) {
-      for (int v = u + 2; v < u + 4 && v < units && ok; ++v) ok = issue_s(v);
-      for (int v = u; v < u + 2 && v < units && ok; ++v) ok = issue_o(v);
-    }
-    if (lane == 0) {  // no MMA may still be writing TMEM when it is released
-      tc_commit(&ctl->drain);
-      mbar_wait(&ctl->drain, 0, nullptr, a.err, kErrTc + 6);
-    }
-  } else {
+  if (warp < 8) {
+    reg_alloc<208>();
     // ---------------- softmax ----------------
     const int g = warp >> 2, qd = warp & 3;
     const int r = qd * 32 + lane;  // TMEM lane
@@ -688,7 +589,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       fence_proxy_async_smem();
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl->q_full);
+    if (lane == 0) {
+      ctl->idle[warp] = idle;
+      mbar_arrive(&ctl->q_full);
+    }
+    named_barrier_sync(1, kTcSoftThreads);
+    // The two warps of an SM quarter take turns at the exponentials, so that one's fill the
+    // other's loads, maxima and hand-overs; a warp without rows needs no turn.
+    const bool turns = !idle && !ctl->idle[warp ^ 4];
 
     float m = -INFINITY, l = 0.0f;  // m: score that weights refer to, unscaled
     const int mine = g < units ? (units - g + 1) / 2 : 0;  // this group's units
@@ -742,19 +650,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       const bool rescale = i > 0 && __any_sync(~0u, grown);
       const float ms = safe_max(m) * kScale2;
-      float sum[4] = {};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float x = ex2(fmaf(__uint_as_float(s[c][2 * k]), kScale2, -ms));
-          const float y = ex2(fmaf(__uint_as_float(s[c][2 * k + 1]), kScale2, -ms));
-          sum[2 * (k & 1)] += x;
-          sum[2 * (k & 1) + 1] += y;
-          s[c][k] = pack_bf2(x, y);
-        }
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       ok = last_done();
       if (!ok) break;
       tc_fence_after();
@@ -769,16 +664,54 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_st_32x32b_x32(trow + kColO + 32 * c, o);
         }
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      if (turns && (g == 1 || i > 0)) {
+        ok = __all_sync(~0u, mbar_wait(&ctl->turn[g][qd], (i - 1 + g) & 1, abort_flag, a.err,
+                                       kErrTc + 11));
+        if (!ok) break;
+      }
+      // Weights, 32 keys at a time: the exponentials of a chunk are issued between the scaling of
+      // the next chunk and the sums and packing of the last, whose results have arrived by then
+      // (a warp issues in order and would otherwise wait for each).
+      float sum[4] = {};
+      auto scale = [&](int c, int k) {
+        s[c][k] = __float_as_uint(fmaf(__uint_as_float(s[c][k]), kScale2, -ms));
+      };
+      auto take = [&](int c, int k) {  // keys k, k + 1
+        const float x = __uint_as_float(s[c][k]), y = __uint_as_float(s[c][k + 1]);
+        sum[k & 2] += x;
+        sum[(k & 2) + 1] += y;
+        s[c][k / 2] = pack_bf2(x, y);
+      };
+      auto store = [&](int c) {  // chunks c - 1 and c
         uint32_t p[32];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          p[k] = s[2 * c][k];
-          p[16 + k] = s[2 * c + 1][k];
+          p[k] = s[c - 1][k];
+          p[16 + k] = s[c][k];
         }
-        tmem_st_32x32b_x32(trow + kColP + 32 * c, p);
+        tmem_st_32x32b_x32(trow + kColP + 16 * (c - 1), p);
+      };
+#pragma unroll
+      for (int k = 0; k < 32; ++k) scale(0, k);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          s[c][k] = __float_as_uint(ex2(__uint_as_float(s[c][k])));
+          s[c][k + 1] = __float_as_uint(ex2(__uint_as_float(s[c][k + 1])));
+          if (c < 3) {
+            scale(c + 1, k);
+            scale(c + 1, k + 1);
+          }
+          if (c > 0) take(c - 1, k);
+        }
+        if (c == 2) store(1);
       }
+      if (turns && lane == 0) mbar_arrive(&ctl->turn[g ^ 1][qd]);
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) take(3, k);
+      store(3);
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -842,6 +775,113 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (row.m >= 0 && !a.direct) a.ml[at] = make_float2(m_all, l_all);
     }
+  } else {
+    reg_dealloc<88>();
+  if (warp == kTcTmaWarp) {
+    // ---------------- TMA: lane i < 2 * boxes issues one box of a block ----------------
+    const int box = min(1 << a.page_shift, kStageKeys);  // rows
+    const int boxes = kTcKeys / box;
+    const bool act = lane < 2 * boxes;
+    const bool is_v = lane >= boxes;
+    const int bx = is_v ? lane - boxes : lane;
+    auto entry = [&](int j) -> int {  // page of this lane's box, n_pages: reads as zeros
+      const int pos = it.k0 + j * kTcKeys + bx * box;
+      if (!act || pos >= it.k1) return a.n_pages;
+      const int k = pos >> a.page_shift;
+      int p = -1;
+      if (pos < a.n_shared) p = a.shared[k];
+      else if (k < a.max_pages) p = a.table[(int64_t)it.b * a.max_pages + k];
+      if (p < 0 || p >= a.n_pages) {
+        report_error(a.err, kErrEntry);
+        p = a.n_pages;
+      }
+      return p;
+    };
+    int p = blocks ? entry(0) : 0;
+    int n = 0;
+    for (; n < blocks; ++n) {
+      const int next = n + 1 < blocks ? entry(n + 1) : 0;
+      const int st = n % kTcStages;
+      bool ok = true;
+      if (n >= kTcStages)
+        ok = mbar_wait(&ctl->kv_empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag, a.err, kErrTc);
+      if (!__all_sync(~0u, ok)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&ctl->kv_full[st], 2 * kTcTile);
+      __syncwarp();
+      if (act) {
+        const int pos = it.k0 + n * kTcKeys + bx * box;
+        const int y = (it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+        tma_load_3d(sKV + (st * 2 + is_v) * kTcTile + bx * box * 128, is_v ? &tmV : &tmK,
+                    &ctl->kv_full[st], 0, y, p);
+      }
+      p = next;
+    }
+    if (n == blocks && v_cut) {
+      // rows of the last page that hold nothing yet: 0 * V must stay 0
+      const int j = blocks - 1, st = j % kTcStages;
+      if (mbar_wait(&ctl->kv_full[st], (j / kTcStages) & 1, abort_flag, a.err, kErrTc + 1)) {
+        uint8_t *v = sKV + (st * 2 + 1) * kTcTile;
+        for (int x = (it.n_valid - it.k0 - j * kTcKeys) * 8 + lane; x < kTcKeys * 8; x += 32)
+          *reinterpret_cast<uint4 *>(v + x * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->v_ready);
+      }
+    }
+    if (*abort_flag)  // no copy may still be writing shared memory when the CTA exits
+      for (int i = n > kTcStages ? n - kTcStages : 0; i < n; ++i)
+        mbar_wait(&ctl->kv_full[i % kTcStages], (i / kTcStages) & 1, nullptr, a.err, kErrTc + 1);
+  } else if (warp == kTcMmaWarp) {
+    // ---------------- MMA: one thread ----------------
+    if (elect_one()) {
+      const uint32_t idS = make_idesc(1, 1, kTileRows, kTcKeys);
+      const uint32_t idO = make_idesc_bmn(1, 1, kTileRows, kPageHd);
+      const uint64_t q_desc = make_sw128_desc(smem_u32(sQ));
+      const uint64_t k_desc = make_sw128_desc(smem_u32(sKV));
+      const uint64_t v_desc = make_sw128_mn_desc(smem_u32(sKV) + kTcTile);
+      bool ok = mbar_wait(&ctl->q_full, 0, abort_flag, a.err, kErrTc + 2);
+      int seen = 0;  // blocks known to be in shared memory
+      auto issue_s = [&](int u) -> bool {
+        const int g = u & 1, i = u >> 1, j = one ? u : i;  // group, its unit, block
+        if (i > 0 && !mbar_wait(&ctl->s_free[g], (i - 1) & 1, abort_flag, a.err, kErrTc + 3))
+          return false;
+        const int st = j % kTcStages;
+        if (j >= seen) {
+          if (!mbar_wait(&ctl->kv_full[st], (j / kTcStages) & 1, abort_flag, a.err, kErrTc + 4))
+            return false;
+          seen = j + 1;
+        }
+        tc_fence_after();
+        tc_mma_bf16_x4(tmem + g * kColGroup + kColS, q_desc + (one ? 0 : g) * (kTcTile >> 4),
+                       k_desc + st * (2 * kTcTile >> 4), idS);
+        tc_commit(&ctl->s_full[g]);
+        return true;
+      };
+      auto issue_o = [&](int u) -> bool {
+        const int g = u & 1, i = u >> 1, j = one ? u : i;
+        if (!mbar_wait(&ctl->p_full[g], i & 1, abort_flag, a.err, kErrTc + 5)) return false;
+        if (v_cut && j == blocks - 1 &&
+            !mbar_wait(&ctl->v_ready, 0, abort_flag, a.err, kErrTc + 10))
+          return false;
+        tc_fence_after();
+        const uint32_t base = tmem + g * kColGroup;
+        tc_mma_bf16_ta_x8(base + kColO, base + kColP, v_desc + (j % kTcStages) * (2 * kTcTile >> 4),
+                          idO, i > 0);
+        tc_commit(&ctl->o_done[g]);
+        if (one || g == 1) tc_commit(&ctl->kv_empty[j % kTcStages]);
+        return true;
+      };
+      for (int u = 0; u < 2 && u < units && ok; ++u) ok = issue_s(u);
+      for (int u = 0; u < units && ok; u += 2) {
+        for (int v = u + 2; v < u + 4 && v < units && ok; ++v) ok = issue_s(v);
+        for (int v = u; v < u + 2 && v < units && ok; ++v) ok = issue_o(v);
+      }
+      // no MMA may still be writing TMEM when it is released
+      tc_commit(&ctl->drain);
+      mbar_wait(&ctl->drain, 0, nullptr, a.err, kErrTc + 6);
+    }
+    __syncwarp();
+  }
   }
   tc_fence_before();
   __syncthreads();
