@@ -24,17 +24,32 @@ namespace w8a8 {
 namespace {
 
 constexpr int kSms = 148;            // the plan below is made for this many SMs
+constexpr float kMaxSlack = 8.0f;    // see grown()
 constexpr float kScale2 = 0.125f * 1.44269504088896340736f;  // log2(e) / sqrt(64)
 constexpr int kErrEntry = 0x1601;    // a table entry outside the pool
-constexpr int kErrWaitFull = 0x1602, kErrWaitEmpty = 0x1603;
+constexpr int kErrWaitFull = 0x1602;
 
 constexpr int kStageKeys = 64;
-constexpr int kStages = 5;
+constexpr int kStages = 2;                         // of each warp
 constexpr uint32_t kTileBytes = kStageKeys * 128;  // keys or values of a stage
-constexpr int kMmaWarps = 4;                       // 16 keys of a stage each
-constexpr int kMmaThreads = kMmaWarps * 32 + 32;   // + the TMA warp
+constexpr int kMmaWarps = 6;                       // one CTA an SM, a warp an item
 constexpr int kRows = 16;                          // query rows of an item
-constexpr int kOPitch = 68;                        // floats a row of the join buffer
+
+// Division of 0 <= n < 2^31 by a fixed d >= 1: for d > 1 with 2^s < d <= 2^(s+1), the
+// quotient is the high word of n * ceil(2^(32+s) / d), shifted by s (Granlund and
+// Montgomery's division by invariant integers).
+struct Div {
+  uint32_t mul, shift;
+};
+Div make_div(uint32_t d) {
+  if (d <= 1) return {0, 0};
+  uint32_t s = 0;
+  while ((2ull << s) < d) ++s;
+  return {(uint32_t)(((1ull << (32 + s)) + d - 1) / d), s};
+}
+__device__ __forceinline__ int quot(int n, const Div &d) {
+  return d.mul ? (int)(__umulhi((uint32_t)n, d.mul) >> d.shift) : n;
+}
 
 struct ApArgs {
   const uint16_t *Q;
@@ -44,9 +59,10 @@ struct ApArgs {
   const int32_t *table, *n_ctx, *n_new, *shared;
   int max_pages, n_pages, page_shift;
   int n_seq, T, g, n_kv, max_ctx, n_shared;
-  // 16-row items: prefix [n_kv][p_tiles][p_splits], then tails
-  // [n_seq][n_kv][t_tiles][t_splits]; slots of a row: p_splits of the first kind
-  // of item, whichever kernel runs it, then t_splits of tails
+  // 16-row items: prefix [p_splits][n_kv][p_tiles], then tails
+  // [t_splits][n_seq][n_kv][t_tiles] (first chunks first: later ones may be empty);
+  // slots of a row: p_splits of the first kind of item, whichever kernel runs it,
+  // then t_splits of tails
   int p_tiles, p_splits, p_chunk;
   int t_tiles, t_splits, t_chunk;
   // tensor-core items (see attention_pages_tc_kernel)
@@ -57,6 +73,7 @@ struct ApArgs {
   int p_end;           // the first kind's items cover positions below this
   int direct;      // one slot a row: the item writes O itself
   int64_t rows;    // n_seq * T * n_head
+  Div by_g, by_T, by_kv, by_head, by_seq_n, by_pt, by_tt;  // g .. n_seq, p_tiles, t_tiles
   float *Op;       // [slot][rows][64]
   float2 *ml;      // [slot][rows]  maximum (base 2), sum
   int *err;
@@ -79,35 +96,44 @@ __device__ __forceinline__ int seq_new(const ApArgs &a, int b) {
   return a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
 }
 
-__device__ __forceinline__ Item get_item(const ApArgs &a, int64_t idx) {
+// Item idx without its key range and its sequence's length.
+__device__ __forceinline__ Item get_item_place(const ApArgs &a, int idx, int *chunk) {
   Item it;
-  const int64_t n_pre = (int64_t)a.n_kv * a.p_tiles * a.p_splits;
+  const int n_pre = a.n_kv * a.p_tiles * a.p_splits;
   if (idx < n_pre) {
-    const int s = (int)(idx % a.p_splits);
-    const int64_t q = idx / a.p_splits;
+    int q = quot(idx, a.by_pt);
+    it.r0 = (idx - q * a.p_tiles) * kRows;
+    *chunk = quot(q, a.by_kv);
+    it.kvh = q - *chunk * a.n_kv;
     it.b = -1;
-    it.r0 = (int)(q % a.p_tiles) * kRows;
-    it.kvh = (int)(q / a.p_tiles);
-    it.slot = s;
+    it.slot = *chunk;
+    return it;
+  }
+  idx -= n_pre;
+  int q = quot(idx, a.by_tt);
+  it.r0 = (idx - q * a.t_tiles) * kRows;
+  idx = q;
+  q = quot(idx, a.by_kv);
+  it.kvh = idx - q * a.n_kv;
+  *chunk = quot(q, a.by_seq_n);
+  it.b = q - *chunk * a.n_seq;
+  it.slot = a.p_splits + *chunk;
+  return it;
+}
+__device__ __forceinline__ Item get_item(const ApArgs &a, int idx) {
+  int s;
+  Item it = get_item_place(a, idx, &s);
+  if (it.b < 0) {
     it.k0 = s * a.p_chunk;
     it.k1 = min(it.k0 + a.p_chunk, a.n_shared);
     it.n_valid = a.n_shared;
     return it;
   }
-  idx -= n_pre;
-  const int s = (int)(idx % a.t_splits);
-  int64_t q = idx / a.t_splits;
-  const int rt = (int)(q % a.t_tiles);
-  q /= a.t_tiles;
-  it.kvh = (int)(q % a.n_kv);
-  it.b = (int)(q / a.n_kv);
-  it.r0 = rt * kRows;
-  it.slot = a.p_splits + s;
   it.n_valid = seq_len(a, it.b);
   const int nn = seq_new(a, it.b);
   it.k0 = a.n_shared + s * a.t_chunk;
   // the last row of the tile sees furthest
-  const int t_last = min((it.r0 + kRows - 1) / a.g, nn - 1);
+  const int t_last = min(quot(it.r0 + kRows - 1, a.by_g), nn - 1);
   const int end = it.n_valid - nn + t_last + 1;
   it.k1 = it.r0 < nn * a.g ? min(it.k0 + a.t_chunk, end) : it.k0;
   return it;
@@ -117,20 +143,20 @@ __device__ __forceinline__ int item_stages(const Item &it) {
 }
 
 struct Row {
-  int64_t m;  // token row, -1: none
+  int m;  // token row, -1: none
   int h, end;
 };
 // Row R of the (m, g) rows of sequence `seq` (-1: of all) and one key head.
-__device__ __forceinline__ Row get_row(const ApArgs &a, int seq, int kvh, int64_t R) {
+__device__ __forceinline__ Row get_row(const ApArgs &a, int seq, int kvh, int R) {
   Row w;
-  w.m = R / a.g;
-  w.h = kvh * a.g + (int)(R - w.m * a.g);
-  int b = seq, t = (int)w.m;
+  w.m = quot(R, a.by_g);
+  w.h = kvh * a.g + (R - w.m * a.g);
+  int b = seq, t = w.m;
   if (b < 0) {
-    b = (int)(w.m / a.T);
-    t = (int)(w.m - (int64_t)b * a.T);
+    b = quot(w.m, a.by_T);
+    t = w.m - b * a.T;
   } else {
-    w.m += (int64_t)b * a.T;
+    w.m += b * a.T;
   }
   w.end = 0;
   if (b >= a.n_seq) {
@@ -168,256 +194,294 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// named_barrier_sync that also tells every thread whether any had `pred` set.
-__device__ __forceinline__ bool named_barrier_or(int id, int n, bool pred) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"((uint32_t)pred), "r"(id), "r"(n)
-      : "memory");
-  return any != 0;
-}
 // A maximum to subtract: 0 where nothing has been seen yet.
 __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// The running maximum that a row's weights refer to moves only when the row's
+// maximum has grown by more than 2^8 in the weights: the sums stay far from the
+// ends of fp32's range, and O is rescaled rarely.
+__device__ __forceinline__ bool grown(float top, float m) {
+  return top > m && !((top - m) * kScale2 <= kMaxSlack);
+}
+
 struct MmaSmem {
-  uint64_t full[kStages], empty[kStages];
-  int abort_flag;
-  float m[kMmaWarps][kRows], l[kMmaWarps][kRows];
-  alignas(16) float O[kMmaWarps][kRows][kOPitch];  // read and written in pairs
+  uint64_t full[kMmaWarps][kStages];
 };
+
+// A warp's items in order, the empty ones left out: each lane looks at one of
+// the next 32 (their lengths come from memory, one round trip for all).
+struct Cursor {
+  int base;         // index of lane 0's item
+  uint32_t left;    // lanes whose items are still to come
+  int k0, k1, n_valid;  // this lane's item
+  Item it;          // the current one
+  int stage, stages;
+};
+
+__device__ __forceinline__ void cursor_next_item(const ApArgs &a, Cursor &c, int step,
+                                                 int n_item, int lane) {
+  c.stage = 0;
+  c.stages = 0;
+  while (c.left == 0) {
+    c.base += 32 * step;
+    if (c.base >= n_item) return;  // stages == 0: no more
+    const int64_t idx = c.base + (int64_t)lane * step;
+    c.k0 = c.k1 = 0;
+    if (idx < n_item) {
+      const Item it = get_item(a, (int)idx);
+      c.k0 = it.k0;
+      c.k1 = it.k1;
+      c.n_valid = it.n_valid;
+    }
+    c.left = __ballot_sync(~0u, idx < n_item && (c.k1 > c.k0 || a.direct));
+  }
+  const int l = __ffs(c.left) - 1;
+  c.left &= c.left - 1;
+  int chunk;
+  c.it = get_item_place(a, c.base + l * step, &chunk);
+  c.it.k0 = __shfl_sync(~0u, c.k0, l);
+  c.it.k1 = __shfl_sync(~0u, c.k1, l);
+  c.it.n_valid = __shfl_sync(~0u, c.n_valid, l);
+  c.stages = max(1, item_stages(c.it));  // (an item without keys, to write zeros: one)
+}
 
 }  // namespace
 
+// What a warp holds of an item: rows lane / 4 and lane / 4 + 8 of 16.
+struct MmaState {
+  uint32_t q[4][4];       // Q, by 16 dims
+  float o[8][4];          // O, by 8 dims
+  float m[2], l[2];       // reference of the weights (a score), this lane's sums
+};
+
+// 64 keys: S = Q K^T, weights, O += P V. HI: rows 8..15 hold anything.
+// lim: keys of this stage that the rows see.
+template <bool HI>
+__device__ __forceinline__ void mma_stage(MmaState &w, uint32_t kb, uint32_t vb,
+                                          const int (&lim)[2], int lane) {
+  constexpr int R = HI ? 2 : 1;
+  const int lm = lane >> 3, lr = lane & 7;
+  const uint32_t krow = kb + ((lm >> 1) * 8 + lr) * 128;  // K: matrices (key half, dim half)
+  const uint32_t vrow = vb + ((lm & 1) * 8 + lr) * 128;   // V: matrices (dim half, key half)
+  float c[8][4] = {};
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    const uint32_t at = krow + (((ks * 2 + (lm & 1)) ^ lr) << 4);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {  // 16 keys
+      uint32_t b[4];
+      ldsm4(at + h * 2048, b);
+      mma16816(c[2 * h], w.q[ks], b[0], b[1]);
+      mma16816(c[2 * h + 1], w.q[ks], b[2], b[3]);
+    }
+  }
+  if (__any_sync(~0u, lim[0] < kStageKeys || (HI && lim[1] < kStageKeys))) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if ((j >> 1) * 8 + (j & 1) + (lane & 3) * 2 >= lim[r])
+          c[j >> 1][2 * r + (j & 1)] = -INFINITY;
+  }
+  bool up[2] = {};
+  float f[2] = {1.0f, 1.0f};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float t0 = fmaxf(c[0][2 * r], c[0][2 * r + 1]), t1 = fmaxf(c[1][2 * r], c[1][2 * r + 1]);
+#pragma unroll
+    for (int j = 2; j < 8; j += 2) {
+      t0 = fmaxf(t0, fmaxf(c[j][2 * r], c[j][2 * r + 1]));
+      t1 = fmaxf(t1, fmaxf(c[j + 1][2 * r], c[j + 1][2 * r + 1]));
+    }
+    float t = fmaxf(t0, t1);
+    t = fmaxf(t, __shfl_xor_sync(~0u, t, 1));
+    t = fmaxf(t, __shfl_xor_sync(~0u, t, 2));
+    up[r] = grown(t, w.m[r]);
+    if (up[r]) {
+      f[r] = ex2((w.m[r] - t) * kScale2);
+      w.m[r] = t;
+    }
+  }
+  if (__any_sync(~0u, up[0] || up[1])) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      w.l[r] *= f[r];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        w.o[d][2 * r] *= f[r];
+        w.o[d][2 * r + 1] *= f[r];
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float ms = safe_max(w.m[r]) * kScale2;
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = ex2(fmaf(c[j][2 * r], kScale2, -ms));
+      const float y = ex2(fmaf(c[j][2 * r + 1], kScale2, -ms));
+      s0 += x;
+      s1 += y;
+      c[j][2 * r] = __uint_as_float(pack_bf2(x, y));
+    }
+    w.l[r] += s0 + s1;
+  }
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const uint32_t pa[4] = {__float_as_uint(c[2 * h][0]), HI ? __float_as_uint(c[2 * h][2]) : 0u,
+                            __float_as_uint(c[2 * h + 1][0]),
+                            HI ? __float_as_uint(c[2 * h + 1][2]) : 0u};
+#pragma unroll
+    for (int d2 = 0; d2 < 4; ++d2) {
+      uint32_t b[4];
+      ldsm4t(vrow + h * 2048 + (((d2 * 2 + (lm >> 1)) ^ lr) << 4), b);
+      mma16816(w.o[2 * d2], pa, b[0], b[1]);
+      mma16816(w.o[2 * d2 + 1], pa, b[2], b[3]);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Items of 16 rows on mma.sync: four warps take 16 keys each of every 64-key
-// stage (TMA, 128-byte swizzle), each with its own running maximum, sum and
-// O, joined through shared memory at the item's end. For the tails a row tile
-// holds the few rows of one sequence and key head, and the keys are read once:
-// the kernel is bound by HBM, and five 16 KB stages on two CTAs an SM cover
-// its latency. The CTAs are persistent, so the TMA warp fetches the next
-// item's keys while the last one is joined.
+// Items of 16 rows on mma.sync, a warp each: for the tails, whose row tile holds
+// the few rows of one sequence and key head, and for a prefix that few rows
+// share. Bound by HBM in principle (23 bytes a cycle and SM: 64 keys of a head,
+// 16 KB, in 700 cycles), by issue and latency in practice. So the warps work
+// alone, with no barrier between them, each with two 64-key stages that it
+// fills itself by TMA (128-byte swizzle), one ahead, across the ends of items.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(kMmaThreads, 2)
+__global__ void __launch_bounds__(kMmaWarps * 32, 1)
     attention_pages_mma_kernel(const __grid_constant__ CUtensorMap tmK,
-                               const __grid_constant__ CUtensorMap tmV, ApArgs a,
-                               int64_t n_item) {
+                               const __grid_constant__ CUtensorMap tmV,
+                               const __grid_constant__ ApArgs a, int n_item) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *sK = smem, *sV = smem + kStages * kTileBytes;
-  MmaSmem *ctl = reinterpret_cast<MmaSmem *>(sV + kStages * kTileBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&ctl->full[i], 1);
-      mbar_init(&ctl->empty[i], kMmaWarps);
-    }
-    ctl->abort_flag = 0;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  uint8_t *ring = smem + warp * (kStages * 2 * kTileBytes);
+  MmaSmem *ctl = reinterpret_cast<MmaSmem *>(smem + kMmaWarps * kStages * 2 * kTileBytes);
+  uint64_t *full = ctl->full[warp];
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
-    prefetch_tmap(&tmK);
-    prefetch_tmap(&tmV);
+    if (warp == 0) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
   }
-  __syncthreads();
-  volatile int *abort_flag = &ctl->abort_flag;
+  __syncwarp();
   pdl_launch_dependents();
   pdl_wait();
 
-  if (warp == kMmaWarps) {
-    // ---------------- TMA: lane i < 2 * boxes issues one box of a stage ----------------
-    const int box = min(1 << a.page_shift, kStageKeys);  // rows
-    const int boxes = kStageKeys / box;
-    const bool act = lane < 2 * boxes;
-    const bool is_v = lane >= boxes;
-    const int bx = is_v ? lane - boxes : lane;
-    uint32_t n = 0;  // stages issued
-    for (int64_t idx = blockIdx.x; idx < n_item; idx += gridDim.x) {
-      const Item it = get_item(a, idx);
-      const int ns = item_stages(it);
-      auto entry = [&](int s) -> int {  // page of this lane's box, n_pages: reads as zeros
-        const int pos = it.k0 + s * kStageKeys + bx * box;
-        if (!act || pos >= it.k1) return a.n_pages;
-        const int k = pos >> a.page_shift;
-        int p = -1;
-        if (it.b < 0) p = a.shared[k];
-        else if (k < a.max_pages) p = a.table[(int64_t)it.b * a.max_pages + k];
-        if (p < 0 || p >= a.n_pages) {
-          report_error(a.err, kErrEntry);
-          p = a.n_pages;
-        }
-        return p;
-      };
-      int p = ns ? entry(0) : 0;
-      for (int s = 0; s < ns; ++s, ++n) {
-        const int next = s + 1 < ns ? entry(s + 1) : 0;
-        const int st = n % kStages;
-        bool ok = true;
-        if (n >= kStages)
-          ok = mbar_wait(&ctl->empty[st], ((n / kStages) & 1) ^ 1, abort_flag, a.err,
-                         kErrWaitEmpty);
-        if (!__all_sync(~0u, ok)) goto drain;
-        if (lane == 0) mbar_arrive_expect_tx(&ctl->full[st], 2 * kTileBytes);
-        __syncwarp();
-        if (act) {
-          const int pos = it.k0 + s * kStageKeys + bx * box;
-          const int y = (it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-          tma_load_3d((is_v ? sV : sK) + st * kTileBytes + bx * box * 128, is_v ? &tmV : &tmK,
-                      &ctl->full[st], 0, y, p);
-        }
-        p = next;
-      }
-    }
-  drain:
-    if (*abort_flag) {
-      // no copy may still be writing shared memory when the CTA exits
-      for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i)
-        mbar_wait(&ctl->full[i % kStages], (i / kStages) & 1, nullptr, a.err, kErrWaitFull);
-    }
-    return;
-  }
+  // neighbouring items (chunks of one row tile, heads of one sequence) on different SMs
+  const int step = gridDim.x * kMmaWarps;
+  const int first = warp * gridDim.x + blockIdx.x - 32 * step;
+  Cursor ld = {}, cp = {};
+  ld.base = cp.base = first;
+  cursor_next_item(a, ld, step, n_item, lane);
+  cp = ld;
 
-  // ---------------- the four mma warps ----------------
-  const int kw = warp * 16;  // this warp's keys of a stage
-  // shared-memory offsets of the ldmatrix rows (128-byte swizzle)
-  const int lm = lane >> 3, lr = lane & 7;
-  const int krow = kw + (lm >> 1) * 8 + lr;  // K: matrices (key half, dim half)
-  const int vrow = kw + (lm & 1) * 8 + lr;   // V: matrices (dim half, key half)
+  // ---- loading: lane i < 2 * boxes brings one box (16 or 32 rows) of a stage ----
+  const int box = min(1 << a.page_shift, kStageKeys);
+  const int boxes = kStageKeys / box;
+  const bool act = lane < 2 * boxes, is_v = lane >= boxes;
+  const int bx = is_v ? lane - boxes : lane;
+  auto entry = [&]() -> int {  // page of this lane's box, n_pages: reads as zeros
+    const int pos = ld.it.k0 + ld.stage * kStageKeys + bx * box;
+    if (!act || ld.stages == 0 || pos >= ld.it.k1) return a.n_pages;
+    const int k = pos >> a.page_shift;
+    int p = -1;
+    if (ld.it.b < 0) p = a.shared[k];
+    else if (k < a.max_pages) p = a.table[(int64_t)ld.it.b * a.max_pages + k];
+    if (p < 0 || p >= a.n_pages) {
+      report_error(a.err, kErrEntry);
+      p = a.n_pages;
+    }
+    return p;
+  };
+  int page = entry();
+  uint32_t loaded = 0;
+  auto load = [&]() {
+    if (ld.stages == 0) return;
+    const int st = loaded % kStages;
+    if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * kTileBytes);
+    __syncwarp();
+    if (act) {
+      const int pos = ld.it.k0 + ld.stage * kStageKeys + bx * box;
+      const int y = (ld.it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+      tma_load_3d(ring + (st * 2 + is_v) * kTileBytes + bx * box * 128, is_v ? &tmV : &tmK,
+                  &full[st], 0, y, page);
+    }
+    ++loaded;
+    if (++ld.stage == ld.stages) cursor_next_item(a, ld, step, n_item, lane);
+    page = entry();
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) load();
+
   uint32_t n = 0;
-  for (int64_t idx = blockIdx.x; idx < n_item; idx += gridDim.x) {
-    const Item it = get_item(a, idx);
-    const int ns = item_stages(it);
-    if (ns == 0 && !a.direct) continue;
+  while (cp.stages > 0) {
+    const Item &it = cp.it;
     const Row row[2] = {get_row(a, it.b, it.kvh, it.r0 + (lane >> 2)),
                         get_row(a, it.b, it.kvh, it.r0 + (lane >> 2) + 8)};
-    uint32_t q[4][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Row &w = row[i & 1];
-        q[ks][i] = w.m < 0 ? 0u
-                           : *reinterpret_cast<const uint32_t *>(
-                                 a.Q + w.m * a.ldq + w.h * kPageHd + ks * 16 + (i >> 1) * 8 +
-                                 (lane & 3) * 2);
-      }
-    float o[8][4] = {};
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    bool ok = true;
-    for (int s = 0; s < ns; ++s, ++n) {
-      const int st = n % kStages;
-      if (!mbar_wait(&ctl->full[st], (n / kStages) & 1, abort_flag, a.err, kErrWaitFull)) {
-        ok = false;
-        break;
-      }
-      const int key0 = it.k0 + s * kStageKeys + kw;
-      const uint32_t kb = smem_u32(sK + st * kTileBytes), vb = smem_u32(sV + st * kTileBytes);
-      if (key0 + 16 > it.n_valid) {
-        // rows of the last page that hold nothing yet: 0 * V must stay 0
-        const int first = max(it.n_valid - key0, 0);
-        for (int u = first * 8 + lane; u < 16 * 8; u += 32)
-          *reinterpret_cast<uint4 *>(sV + st * kTileBytes + (kw + (u >> 3)) * 128 +
-                                     (u & 7) * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      float c[2][4] = {};
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        uint32_t b[4];
-        ldsm4(kb + krow * 128 + (((ks * 2 + (lm & 1)) ^ (krow & 7)) << 4), b);
-        mma16816(c[0], q[ks], b[0], b[1]);
-        mma16816(c[1], q[ks], b[2], b[3]);
-      }
-      float p[2][4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {  // rows lane/4 and lane/4 + 8
-        float t = mx[r];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = key0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
-          float x = c[j >> 1][2 * r + (j & 1)] * kScale2;
-          x = key < min(row[r].end, it.k1) ? x : -INFINITY;
-          p[r][j] = x;
-          t = fmaxf(t, x);
-        }
-        t = fmaxf(t, __shfl_xor_sync(~0u, t, 1));
-        t = fmaxf(t, __shfl_xor_sync(~0u, t, 2));
-        const float ms = safe_max(t), f = ex2(mx[r] - ms);
-        mx[r] = t;
-        sum[r] *= f;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          o[d][2 * r] *= f;
-          o[d][2 * r + 1] *= f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          p[r][j] = ex2(p[r][j] - ms);
-          sum[r] += p[r][j];
-        }
-      }
-      const uint32_t pa[4] = {pack_bf2(p[0][0], p[0][1]), pack_bf2(p[1][0], p[1][1]),
-                              pack_bf2(p[0][2], p[0][3]), pack_bf2(p[1][2], p[1][3])};
-#pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2) {
-        uint32_t b[4];
-        ldsm4t(vb + vrow * 128 + (((d2 * 2 + (lm >> 1)) ^ (vrow & 7)) << 4), b);
-        mma16816(o[2 * d2], pa, b[0], b[1]);
-        mma16816(o[2 * d2 + 1], pa, b[2], b[3]);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->empty[st]);
-    }
-    // ---- join the four warps ----
+    const bool hi = __any_sync(~0u, row[1].m >= 0);
+    MmaState w = {};
+    w.m[0] = w.m[1] = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
-      sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
-      const int rr = (lane >> 2) + 8 * r;
-      if ((lane & 3) == 0) {
-        ctl->m[warp][rr] = mx[r];
-        ctl->l[warp][rr] = sum[r];
-      }
+      if (row[r].m < 0) continue;
+      const uint32_t *src = reinterpret_cast<const uint32_t *>(a.Q + (int64_t)row[r].m * a.ldq +
+                                                               row[r].h * kPageHd) + (lane & 3);
 #pragma unroll
-      for (int d = 0; d < 8; ++d)
-        *reinterpret_cast<float2 *>(&ctl->O[warp][rr][d * 8 + (lane & 3) * 2]) =
-            make_float2(o[d][2 * r], o[d][2 * r + 1]);
-    }
-    if (named_barrier_or(1, kMmaWarps * 32, !ok)) return;  // a wait ran out in some warp
-    {
-      const int r = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * 8;
-      const Row w = get_row(a, it.b, it.kvh, it.r0 + r);
-      if (w.m >= 0) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kMmaWarps; ++i) m = fmaxf(m, ctl->m[i][r]);
-        const float ms = safe_max(m);
-        float l = 0.0f, acc[8] = {};
-#pragma unroll
-        for (int i = 0; i < kMmaWarps; ++i) {
-          const float f = ex2(ctl->m[i][r] - ms);
-          l += f * ctl->l[i][r];
-#pragma unroll
-          for (int d = 0; d < 8; ++d) acc[d] += f * ctl->O[i][r][d0 + d];
-        }
-        if (a.direct) {
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          uint32_t *dst = reinterpret_cast<uint32_t *>(a.O + w.m * a.ldo + w.h * kPageHd + d0);
-#pragma unroll
-          for (int d = 0; d < 4; ++d) dst[d] = pack_bf2(acc[2 * d] * inv, acc[2 * d + 1] * inv);
-        } else {
-          const int64_t at = (int64_t)it.slot * a.rows + w.m * (a.n_kv * a.g) + w.h;
-          float4 *dst = reinterpret_cast<float4 *>(a.Op + at * kPageHd + d0);
-          dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-          dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-          if (d0 == 0) a.ml[at] = make_float2(m, l);
-        }
+      for (int ks = 0; ks < 4; ++ks) {
+        w.q[ks][r] = src[ks * 8];
+        w.q[ks][r + 2] = src[ks * 8 + 4];
       }
     }
-    named_barrier_sync(1, kMmaWarps * 32);
+    for (int s = 0; s < cp.stages; ++s, ++n) {
+      load();  // into the stage that was read last
+      const int st = n % kStages;
+      if (!__all_sync(~0u, mbar_wait(&full[st], (n / kStages) & 1, nullptr, a.err, kErrWaitFull))) {
+        // no copy may still be writing shared memory when the warp exits
+        for (uint32_t i = n + 1; i < loaded; ++i)
+          mbar_wait(&full[i % kStages], (i / kStages) & 1, nullptr, a.err, kErrWaitFull);
+        return;
+      }
+      const int key0 = it.k0 + s * kStageKeys;
+      uint8_t *sK = ring + st * 2 * kTileBytes, *sV = sK + kTileBytes;
+      if (key0 + kStageKeys > it.n_valid) {
+        // rows of the last page that hold nothing yet: 0 * V must stay 0
+        for (int u = max(it.n_valid - key0, 0) * 8 + lane; u < kStageKeys * 8; u += 32)
+          *reinterpret_cast<uint4 *>(sV + u * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // before the next copy into this stage
+        __syncwarp();
+      }
+      const int lim[2] = {min(row[0].end, it.k1) - key0, min(row[1].end, it.k1) - key0};
+      if (hi) mma_stage<true>(w, smem_u32(sK), smem_u32(sV), lim, lane);
+      else mma_stage<false>(w, smem_u32(sK), smem_u32(sV), lim, lane);
+      __syncwarp();  // reads of this stage, then the copy that the next load() starts into it
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float l = w.l[r];
+      l += __shfl_xor_sync(~0u, l, 1);
+      l += __shfl_xor_sync(~0u, l, 2);
+      if (row[r].m < 0) continue;
+      if (a.direct) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint32_t *dst = reinterpret_cast<uint32_t *>(a.O + (int64_t)row[r].m * a.ldo +
+                                                     row[r].h * kPageHd + (lane & 3) * 2);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          dst[4 * d] = pack_bf2(w.o[d][2 * r] * inv, w.o[d][2 * r + 1] * inv);
+      } else {
+        const int64_t at = it.slot * a.rows + (int64_t)row[r].m * (a.n_kv * a.g) + row[r].h;
+        float2 *dst = reinterpret_cast<float2 *>(a.Op + at * kPageHd + (lane & 3) * 2);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) dst[4 * d] = make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
+        if ((lane & 3) == 0) a.ml[at] = make_float2(w.m[r] * kScale2, l);
+      }
+    }
+    cursor_next_item(a, cp, step, n_item, lane);
   }
 }
 
@@ -436,22 +500,19 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 // the exponentials of this one run, and the groups' MMAs overlap each other's
 // softmax. A single tile (the last rows, or few of them) is worked on by both
 // groups, a block each in turn, which are joined at the end.
-// The running maximum that weights refer to moves only when a row's maximum has
-// grown by more than 2^8 (in the exponent): the sums stay far from the range of
-// fp32, and O is rescaled rarely, by the group itself.
 // Bound by the exponentials: 128 x 128 of them at 16 a cycle are 1024 cycles,
 // the two products of a tile 512.
 // ---------------------------------------------------------------------------
 namespace {
 
 constexpr int kTcKeys = 128;
+constexpr int kBoxRows = 64;  // at most, of a TMA box
 constexpr int kTcStages = 5;
 constexpr uint32_t kTcTile = kTcKeys * 128;  // Q tile, or K or V of a block: 16 KB
 constexpr int kTcTmaWarp = 8, kTcMmaWarp = 9;
 constexpr int kTcThreads = 12 * 32;  // three warpgroups; the last two warps only pass registers
 constexpr int kTcSoftThreads = 8 * 32;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 192, kColGroup = 256;
-constexpr float kMaxSlack = 8.0f;  // base 2
 constexpr int kErrTc = 0x1610;
 
 struct TcCtl {
@@ -468,7 +529,7 @@ struct TcCtl {
 
 struct TcItem {
   int b, kvh;      // sequence, -1: rows of all
-  int64_t r0, r1;  // rows among the (m, g) rows of b, or of all
+  int r0, r1;      // rows among the (m, g) rows of b, or of all
   int slot, k0, k1, n_valid;
 };
 
@@ -483,12 +544,12 @@ __device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx) {
     it.b = q % a.n_seq;
     const int pair = a.pairs - 1 - q / a.n_seq;
     const int nn = seq_new(a, it.b), n = seq_len(a, it.b);
-    it.r0 = (int64_t)pair * kPairRows;
-    it.r1 = min(it.r0 + kPairRows, (int64_t)nn * a.g);
+    it.r0 = pair * kPairRows;
+    it.r1 = min(it.r0 + kPairRows, nn * a.g);
     it.slot = s;
     it.k0 = s * a.p_chunk;
     it.n_valid = n;
-    const int end = it.r1 > it.r0 ? n - nn + (int)((it.r1 - 1) / a.g) + 1 : 0;
+    const int end = it.r1 > it.r0 ? n - nn + (it.r1 - 1) / a.g + 1 : 0;
     it.k1 = min(it.k0 + a.p_chunk, end);
     return it;
   }
@@ -499,8 +560,8 @@ __device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx) {
   const bool one = q >= full;
   const int pair = one ? a.pairs : q / a.full_splits;
   it.slot = one ? q - full : q - pair * a.full_splits;
-  it.r0 = (int64_t)pair * kPairRows;
-  it.r1 = min(it.r0 + kPairRows, (int64_t)a.n_seq * a.T * a.g);
+  it.r0 = pair * kPairRows;
+  it.r1 = min(it.r0 + kPairRows, a.n_seq * a.T * a.g);
   const int chunk = one ? a.one_chunk : a.p_chunk;
   it.k0 = it.slot * chunk;
   it.k1 = min(it.k0 + chunk, a.n_shared);
@@ -508,7 +569,7 @@ __device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx) {
   return it;
 }
 
-__device__ __forceinline__ Row get_tc_row(const ApArgs &a, const TcItem &it, int64_t R) {
+__device__ __forceinline__ Row get_tc_row(const ApArgs &a, const TcItem &it, int R) {
   Row w = get_row(a, it.b, it.kvh, R);
   if (R >= it.r1) {
     w.m = -1;
@@ -521,7 +582,8 @@ __device__ __forceinline__ Row get_tc_row(const ApArgs &a, const TcItem &it, int
 
 __global__ void __launch_bounds__(kTcThreads, 1)
     attention_pages_tc_kernel(const __grid_constant__ CUtensorMap tmK,
-                              const __grid_constant__ CUtensorMap tmV, ApArgs a) {
+                              const __grid_constant__ CUtensorMap tmV,
+                              const __grid_constant__ ApArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t *sQ = smem;                       // [2] tiles
@@ -531,7 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   const TcItem it = get_tc_item(a, blockIdx.x);
-  const int n_rows = (int)(it.r1 - it.r0);
+  const int n_rows = it.r1 - it.r0;
   const int blocks = it.k1 > it.k0 ? (it.k1 - it.k0 + kTcKeys - 1) / kTcKeys : 0;
   // an item without keys: its slot is not read, unless rows get their zeros here
   if (n_rows <= 0 || (blocks == 0 && !a.direct)) return;
@@ -580,7 +642,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // Q row into its swizzled place
     if (!one || g == 0) {
       uint8_t *dst = sQ + g * kTcTile + r * 128;
-      const uint4 *src = reinterpret_cast<const uint4 *>(a.Q + row.m * a.ldq + row.h * kPageHd);
+      const uint4 *src = reinterpret_cast<const uint4 *>(a.Q + (int64_t)row.m * a.ldq + row.h * kPageHd);
       uint4 v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = row.m >= 0 ? src[i] : make_uint4(0, 0, 0, 0);
@@ -641,14 +703,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int k = 1; k < 32; ++k) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][k]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool grown = top > m && !((top - m) * kScale2 <= kMaxSlack);
+      const bool up = grown(top, m);
       float f = 1.0f;
-      if (grown) {
+      if (up) {
         f = ex2((m - top) * kScale2);  // 0 at the first key (m = -inf)
         m = top;
         l *= f;
       }
-      const bool rescale = i > 0 && __any_sync(~0u, grown);
+      const bool rescale = i > 0 && __any_sync(~0u, up);
       const float ms = safe_max(m) * kScale2;
       ok = last_done();
       if (!ok) break;
@@ -741,7 +803,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l_all = f0 * l + f1 * w.y;
       }
       const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
-      const int64_t at = (int64_t)it.slot * a.rows + row.m * (a.n_kv * a.g) + row.h;
+      const int64_t at = it.slot * a.rows + (int64_t)row.m * (a.n_kv * a.g) + row.h;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t o[16], o1[16];
@@ -762,7 +824,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (row.m >= 0) {
           if (a.direct) {
             uint32_t *dst =
-                reinterpret_cast<uint32_t *>(a.O + row.m * a.ldo + row.h * kPageHd + 16 * c);
+                reinterpret_cast<uint32_t *>(a.O + (int64_t)row.m * a.ldo + row.h * kPageHd + 16 * c);
 #pragma unroll
             for (int k = 0; k < 8; ++k) dst[k] = pack_bf2(x[2 * k] * inv, x[2 * k + 1] * inv);
           } else {
@@ -779,7 +841,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     reg_dealloc<88>();
   if (warp == kTcTmaWarp) {
     // ---------------- TMA: lane i < 2 * boxes issues one box of a block ----------------
-    const int box = min(1 << a.page_shift, kStageKeys);  // rows
+    const int box = min(1 << a.page_shift, kBoxRows);
     const int boxes = kTcKeys / box;
     const bool act = lane < 2 * boxes;
     const bool is_v = lane >= boxes;
@@ -892,48 +954,67 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// The join of a row's items, a warp a row (two dims a lane). An item without
-// keys below the row's end was not run: its slot is not read.
+// The join of a row's items, a warp a row: a lane a slot for the weights, then
+// two dims a lane, eight slots' loads in flight. An item without keys below the
+// row's end was not run: its slot counts as weight zero, unread.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) attention_pages_join_kernel(ApArgs a) {
+__global__ void __launch_bounds__(256)
+    attention_pages_join_kernel(const __grid_constant__ ApArgs a) {
   const int lane = threadIdx.x & 31;
-  const int n_head = a.n_kv * a.g;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   pdl_launch_dependents();
   pdl_wait();
   if (row >= a.rows) return;
-  const int64_t m = row / n_head;
-  const int b = (int)(m / a.T), t = (int)(m - (int64_t)b * a.T);
+  const int m = quot(row, a.by_head), h = row - m * (a.n_kv * a.g);
+  const int b = quot(m, a.by_T), t = m - b * a.T;
   const int nn = seq_new(a, b);
   if (t >= nn) return;
   const int end = seq_len(a, b) - nn + t + 1;
   const int slots = a.p_splits + a.t_splits;
   // the row's place among the prefix rows of its key head tells its items' chunk
-  const int64_t R = m * a.g + (int)(row - m * n_head) % a.g;
-  const int p_chunk = a.one_splits && R >= (int64_t)a.pairs * kPairRows ? a.one_chunk : a.p_chunk;
-  auto live = [&](int s) {
-    return s < a.p_splits ? s * (int64_t)p_chunk < min(end, a.p_end)
-                          : a.n_shared + (s - a.p_splits) * (int64_t)a.t_chunk < end;
-  };
-  float mx = -INFINITY;
-  for (int s = lane; s < slots; s += 32)
-    if (live(s)) mx = fmaxf(mx, a.ml[s * a.rows + row].x);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, d));
-  const float ms = safe_max(mx);
-  float l = 0.0f;
+  const int R = m * a.g + (h - quot(h, a.by_g) * a.g);
+  const int p_chunk = a.one_splits && R >= a.pairs * kPairRows ? a.one_chunk : a.p_chunk;
+  float mx = -INFINITY, l = 0.0f;
   float2 acc = make_float2(0.0f, 0.0f);
-  for (int s = 0; s < slots; ++s) {
-    if (!live(s)) continue;
-    const float2 v = a.ml[s * a.rows + row];
-    const float2 x = reinterpret_cast<const float2 *>(a.Op + (s * a.rows + row) * kPageHd)[lane];
-    const float f = ex2(v.x - ms);
-    l += f * v.y;
-    acc.x += f * x.x;
-    acc.y += f * x.y;
+  for (int base = 0; base < slots; base += 32) {
+    const int s = base + lane;
+    const bool live = s < a.p_splits ? (int64_t)s * p_chunk < min(end, a.p_end)
+                                     : s < slots && a.n_shared + (int64_t)(s - a.p_splits) *
+                                                                     a.t_chunk < end;
+    const float2 v = live ? a.ml[s * a.rows + row] : make_float2(-INFINITY, 0.0f);
+    float top = v.x;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    top = fmaxf(top, mx);
+    const float ms = safe_max(top), f = ex2(mx - ms), w = live ? ex2(v.x - ms) : 0.0f;
+    mx = top;
+    l = l * f + w * v.y;  // this lane's slots
+    acc.x *= f;
+    acc.y *= f;
+    for (uint32_t todo = __ballot_sync(~0u, live); todo;) {
+      float2 x[8];
+      float wx[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = todo ? __ffs(todo) - 1 : 0;
+        wx[i] = __shfl_sync(~0u, w, k);
+        if (!todo) wx[i] = 0.0f;
+        x[i] = todo ? reinterpret_cast<const float2 *>(
+                          a.Op + ((base + k) * a.rows + row) * kPageHd)[lane]
+                    : make_float2(0.0f, 0.0f);
+        todo &= todo - 1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        acc.x += wx[i] * x[i].x;
+        acc.y += wx[i] * x[i].y;
+      }
+    }
   }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  reinterpret_cast<uint32_t *>(a.O + m * a.ldo + (row - m * n_head) * kPageHd)[lane] =
+  reinterpret_cast<uint32_t *>(a.O + (int64_t)m * a.ldo + h * kPageHd)[lane] =
       pack_bf2(acc.x * inv, acc.y * inv);
 }
 
@@ -963,7 +1044,7 @@ int chunk_keys(int64_t keys, int64_t groups, int64_t want, int min_keys, int ste
 Plan make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared) {
   Plan p = {};
   const int g = n_head / n_kv;
-  const int64_t want = kSms * 4;  // 16-row items: two waves of two CTAs an SM
+  const int64_t want = kSms * kMmaWarps * 3;  // 16-row items: some for every warp
   const int64_t own = (int64_t)T * g, all = own * n_seq;  // rows of a key head
   p.p_end = n_shared;
   if (own >= 64) {
@@ -1067,6 +1148,13 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_co
   a.one_chunk = p.one_chunk;
   a.p_end = p.p_end;
   a.rows = (int64_t)q.n_seq * q.T * q.n_head;
+  a.by_g = make_div(g);
+  a.by_T = make_div(q.T);
+  a.by_kv = make_div(c.n_kv_head);
+  a.by_head = make_div(q.n_head);
+  a.by_seq_n = make_div(q.n_seq);
+  a.by_pt = make_div(p.p_tiles);
+  a.by_tt = make_div(p.t_tiles);
   const int slots = p.p_splits + p.t_splits;
   a.direct = slots == 1;
   a.Op = reinterpret_cast<float *>(q.ws);
@@ -1075,22 +1163,22 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_co
   DeviceCtx *ctx = device_ctx(&st);
   if (!ctx) return st;
   a.err = ctx->err;
-  const int box = c.page < kStageKeys ? c.page : kStageKeys;
   const int64_t off = (int64_t)q.layer * c.n_kv_head * c.page * kPageHd;
-  const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)c.n_kv_head * c.page;
-  st = make_tmap_3d(&tmK, c.K + off, bf, (uint64_t)c.n_pages, rows, kPageHd, kPageHd * 2,
-                    (uint64_t)c.page_stride * 2, kPageHd, box);
-  if (st) return st;
-  st = make_tmap_3d(&tmV, c.V + off, bf, (uint64_t)c.n_pages, rows, kPageHd, kPageHd * 2,
-                    (uint64_t)c.page_stride * 2, kPageHd, box);
-  if (st) return st;
+  CUtensorMap tmK, tmV;
+  auto maps = [&](int box) {  // of at most `box` rows
+    const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (c.page < box) box = c.page;
+    int e = make_tmap_3d(&tmK, c.K + off, bf, (uint64_t)c.n_pages, rows, kPageHd, kPageHd * 2,
+                         (uint64_t)c.page_stride * 2, kPageHd, box);
+    return e ? e : make_tmap_3d(&tmV, c.V + off, bf, (uint64_t)c.n_pages, rows, kPageHd,
+                                kPageHd * 2, (uint64_t)c.page_stride * 2, kPageHd, box);
+  };
   static bool tc_ready[64], mma_ready[64];
   if (p.tc) {
     const size_t smem = 1024 + (2 + 2 * kTcStages) * kTcTile + sizeof(TcCtl);
     st = opt_in_smem(attention_pages_tc_kernel, smem, tc_ready);
-    if (st) return st;
+    if (st || (st = maps(kBoxRows))) return st;
     launch_pdl(attention_pages_tc_kernel, dim3((unsigned)p.tc_items), dim3(kTcThreads), smem, s,
                tmK, tmV, a);
     st = check_launch("attention_pages_tc");
@@ -1099,12 +1187,12 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_co
   const int64_t items = (int64_t)a.n_kv * p.p_tiles * p.p_splits +
                         (int64_t)a.n_seq * a.n_kv * p.t_tiles * p.t_splits;
   if (items > 0) {
-    const size_t smem = 1024 + 2 * kStages * kTileBytes + sizeof(MmaSmem);
+    const size_t smem = 1024 + kMmaWarps * kStages * 2 * kTileBytes + sizeof(MmaSmem);
     st = opt_in_smem(attention_pages_mma_kernel, smem, mma_ready);
-    if (st) return st;
-    const int64_t grid = items < 2 * sm_count ? items : 2 * sm_count;
-    launch_pdl(attention_pages_mma_kernel, dim3((unsigned)grid), dim3(kMmaThreads), smem, s, tmK,
-               tmV, a, items);
+    if (st || (st = maps(kStageKeys))) return st;
+    const int64_t grid = items < sm_count ? items : sm_count;
+    launch_pdl(attention_pages_mma_kernel, dim3((unsigned)grid), dim3(kMmaWarps * 32), smem, s,
+               tmK, tmV, a, (int)items);
     st = check_launch("attention_pages_mma");
     if (st) return st;
   }
