@@ -710,7 +710,7 @@ extern "C" int w8a8_attention_pages(const w8a8_pages *c, int layer, const gpt2_b
   q.shared = shared_pages;
   q.ws = workspace;
   q.ws_bytes = workspace_bytes;
-  return launch_attention_pages(a, q, sm_count(), (cudaStream_t)stream);
+  return launch_attention_pages(a, q, (cudaStream_t)stream);
 }
 
 extern "C" int w8a8_lm_head(const gpt2_bf16_t *Xf, int64_t ldx, int M, int d,

@@ -34,6 +34,12 @@ constexpr int kStages = 2;                         // of each warp
 constexpr uint32_t kTileBytes = kStageKeys * 128;  // keys or values of a stage
 constexpr int kMmaWarps = 6;                       // one CTA an SM, a warp an item
 constexpr int kRows = 16;                          // query rows of an item
+// A prefix of more 16-row stages than this goes to the tensor-core kernel, if it takes several
+// row tiles. That kernel has a fixed cost of some 8 us; the 16-row kernel, whose re-reads hit
+// L2, gets through about 500 stages a microsecond (64 rows of 4 key heads over 16384 positions,
+// 4096 stages: 25.0 us with it, 20.6 with the other; a single row tile is read once: 8 rows of
+// 16 key heads over 16384 positions, as many stages: 28.6 and 33.0).
+constexpr int kMinTcStages = 4000;
 
 // Division of 0 <= n < 2^31 by a fixed d >= 1: for d > 1 with 2^s < d <= 2^(s+1), the
 // quotient is the high word of n * ceil(2^(32+s) / d), shifted by s (Granlund and
@@ -59,87 +65,38 @@ struct ApArgs {
   const int32_t *table, *n_ctx, *n_new, *shared;
   int max_pages, n_pages, page_shift;
   int n_seq, T, g, n_kv, max_ctx, n_shared;
-  // 16-row items: prefix [p_splits][n_kv][p_tiles], then tails
-  // [t_splits][n_seq][n_kv][t_tiles] (first chunks first: later ones may be empty);
-  // slots of a row: p_splits of the first kind of item, whichever kernel runs it,
-  // then t_splits of tails
-  int p_tiles, p_splits, p_chunk;
-  int t_tiles, t_splits, t_chunk;
+  // groups of the 16-row kernel (a row tile of a key head, and the keys it sees, in
+  // 64-key stages): of the prefix [n_kv][p_tiles] with p_stages each, then of every
+  // sequence [n_kv][its row tiles] over its tail (see Walk)
+  int p_tiles, p_stages;
+  int whole;           // stages given to every sequence's groups, none split; 0: as many as it has
   // tensor-core items (see attention_pages_tc_kernel)
   int by_seq;          // rows of one sequence over all its keys, or of all over the prefix
   int pairs;           // pairs of 128-row tiles: of a sequence, or full ones of all rows
-  int full_splits;     // items over the prefix of a full pair; p_splits: the larger number
-  int one_splits, one_chunk;  // prefix items of a last single tile
-  int p_end;           // the first kind's items cover positions below this
-  int direct;      // one slot a row: the item writes O itself
-  int64_t rows;    // n_seq * T * n_head
-  Div by_g, by_T, by_kv, by_head, by_seq_n, by_pt, by_tt;  // g .. n_seq, p_tiles, t_tiles
-  float *Op;       // [slot][rows][64]
-  float2 *ml;      // [slot][rows]  maximum (base 2), sum
+  int p_splits, p_chunk;      // items and keys of an item; of the prefix of a full pair
+  int one_splits, one_chunk;  // those of a last single tile
+  int p_end;           // these items cover positions below this
+  int behind;          // the 16-row kernel runs behind the tensor-core kernel
+  int direct;          // every row is one item's or group's, which writes O itself
+  int64_t rows;        // n_seq * T * n_head
+  Div by_g, by_T, by_head;
+  // Parts of rows: [slots][rows], one for each tensor-core item over a row's prefix, or one for
+  // its 16-row group over it; one for its group over the tail; then [warps][2][16], of groups
+  // that several warps share: a warp's rows of the group it joined, and of the one it began.
+  int slots;
+  float *Op;           // [part][64]
+  float2 *ml;          // [part] maximum (base 2), sum
+  int *shares;         // [prefix, tail][rows] first warp of the row's group * 2^16 + warps
   int *err;
 };
 
 constexpr int kTileRows = 128, kPairRows = 256;  // tensor-core row tiles
-
-struct Item {
-  int b;       // sequence of a tail, -1: prefix
-  int kvh, r0; // key head; first row of the tile among the (m, g) rows of b or of all
-  int slot;
-  int k0, k1;  // positions
-  int n_valid; // positions that hold anything
-};
 
 __device__ __forceinline__ int seq_len(const ApArgs &a, int b) {
   return min(max(a.n_ctx[b], 0), a.max_ctx);
 }
 __device__ __forceinline__ int seq_new(const ApArgs &a, int b) {
   return a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
-}
-
-// Item idx without its key range and its sequence's length.
-__device__ __forceinline__ Item get_item_place(const ApArgs &a, int idx, int *chunk) {
-  Item it;
-  const int n_pre = a.n_kv * a.p_tiles * a.p_splits;
-  if (idx < n_pre) {
-    int q = quot(idx, a.by_pt);
-    it.r0 = (idx - q * a.p_tiles) * kRows;
-    *chunk = quot(q, a.by_kv);
-    it.kvh = q - *chunk * a.n_kv;
-    it.b = -1;
-    it.slot = *chunk;
-    return it;
-  }
-  idx -= n_pre;
-  int q = quot(idx, a.by_tt);
-  it.r0 = (idx - q * a.t_tiles) * kRows;
-  idx = q;
-  q = quot(idx, a.by_kv);
-  it.kvh = idx - q * a.n_kv;
-  *chunk = quot(q, a.by_seq_n);
-  it.b = q - *chunk * a.n_seq;
-  it.slot = a.p_splits + *chunk;
-  return it;
-}
-__device__ __forceinline__ Item get_item(const ApArgs &a, int idx) {
-  int s;
-  Item it = get_item_place(a, idx, &s);
-  if (it.b < 0) {
-    it.k0 = s * a.p_chunk;
-    it.k1 = min(it.k0 + a.p_chunk, a.n_shared);
-    it.n_valid = a.n_shared;
-    return it;
-  }
-  it.n_valid = seq_len(a, it.b);
-  const int nn = seq_new(a, it.b);
-  it.k0 = a.n_shared + s * a.t_chunk;
-  // the last row of the tile sees furthest
-  const int t_last = min(quot(it.r0 + kRows - 1, a.by_g), nn - 1);
-  const int end = it.n_valid - nn + t_last + 1;
-  it.k1 = it.r0 < nn * a.g ? min(it.k0 + a.t_chunk, end) : it.k0;
-  return it;
-}
-__device__ __forceinline__ int item_stages(const Item &it) {
-  return it.k1 > it.k0 ? (it.k1 - it.k0 + kStageKeys - 1) / kStageKeys : 0;
 }
 
 struct Row {
@@ -173,6 +130,31 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Pairs of fp32 (one instruction for two results).
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ void f2_split(F2 v, float &x, float &y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -208,41 +190,171 @@ struct MmaSmem {
   uint64_t full[kMmaWarps][kStages];
 };
 
-// A warp's items in order, the empty ones left out: each lane looks at one of
-// the next 32 (their lengths come from memory, one round trip for all).
-struct Cursor {
-  int base;         // index of lane 0's item
-  uint32_t left;    // lanes whose items are still to come
-  int k0, k1, n_valid;  // this lane's item
-  Item it;          // the current one
-  int stage, stages;
+// A warp's part of a group.
+struct Item {
+  int b, nn;    // sequence of a tail and its new rows; -1: prefix
+  int kvh, r0;  // key head; first row of the tile among the (m, g) rows of b or of all
+  int k0, k1;   // positions
+  int n_valid;  // positions that hold anything
+  int shares;   // where `begins`: first warp of the group * 2^16 + its warps
+  bool begins, ends;
 };
 
-__device__ __forceinline__ void cursor_next_item(const ApArgs &a, Cursor &c, int step,
-                                                 int n_item, int lane) {
-  c.stage = 0;
-  c.stages = 0;
-  while (c.left == 0) {
-    c.base += 32 * step;
-    if (c.base >= n_item) return;  // stages == 0: no more
-    const int64_t idx = c.base + (int64_t)lane * step;
-    c.k0 = c.k1 = 0;
-    if (idx < n_item) {
-      const Item it = get_item(a, (int)idx);
-      c.k0 = it.k0;
-      c.k1 = it.k1;
-      c.n_valid = it.n_valid;
-    }
-    c.left = __ballot_sync(~0u, idx < n_item && (c.k1 > c.k0 || a.direct));
+// All groups' stages in a row, of which every warp takes an equal stretch: the
+// kernel has no stragglers whatever the sequences' lengths. A walk passes over the
+// sequences 32 at a time, a lane each.
+struct Walk {
+  int left, per_warp, me;         // stages to go, of a stretch; this warp
+  int b, kvh, tile, s0;           // the next group, and its stages already taken
+  int st, tiles, n_valid, nn;     // its stages; its sequence's row tiles, length, new rows
+  int base;                       // sequence of lane 0
+  uint32_t more;                  // lanes with sequences still to come
+  int l_st, l_tiles, l_valid, l_nn;  // this lane's sequence
+};
+
+__device__ __forceinline__ int tail_stages(const ApArgs &a, int n_valid) {
+  if (a.whole) return a.whole;
+  return n_valid > a.n_shared ? (n_valid - a.n_shared + kStageKeys - 1) / kStageKeys : 0;
+}
+__device__ __forceinline__ int row_tiles(const ApArgs &a, int nn) {
+  return (nn * a.g + kRows - 1) / kRows;
+}
+
+__device__ __forceinline__ int all_stages(const ApArgs &a, int lane) {
+  int v = 0;
+#pragma unroll 4
+  for (int b = lane; b < a.n_seq; b += 32)
+    v += tail_stages(a, seq_len(a, b)) * row_tiles(a, seq_new(a, b));
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return (a.p_tiles * a.p_stages + v) * a.n_kv;
+}
+
+// The next 32 sequences; returns this lane's stages.
+__device__ __forceinline__ int walk_batch(const ApArgs &a, Walk &w, int lane) {
+  const int b = w.base + lane;
+  w.l_valid = w.l_nn = w.l_st = 0;
+  if (b < a.n_seq) {
+    w.l_valid = seq_len(a, b);
+    w.l_nn = seq_new(a, b);
+    w.l_st = tail_stages(a, w.l_valid);
   }
-  const int l = __ffs(c.left) - 1;
-  c.left &= c.left - 1;
-  int chunk;
-  c.it = get_item_place(a, c.base + l * step, &chunk);
-  c.it.k0 = __shfl_sync(~0u, c.k0, l);
-  c.it.k1 = __shfl_sync(~0u, c.k1, l);
-  c.it.n_valid = __shfl_sync(~0u, c.n_valid, l);
-  c.stages = max(1, item_stages(c.it));  // (an item without keys, to write zeros: one)
+  w.l_tiles = row_tiles(a, w.l_nn);
+  const int v = w.l_st * w.l_tiles * a.n_kv;
+  w.more = __ballot_sync(~0u, v > 0);
+  return v;
+}
+__device__ __forceinline__ void walk_take_lane(Walk &w, int l) {
+  w.b = w.base + l;
+  w.more &= ~1u << l;
+  w.st = __shfl_sync(~0u, w.l_st, l);
+  w.tiles = __shfl_sync(~0u, w.l_tiles, l);
+  w.n_valid = __shfl_sync(~0u, w.l_valid, l);
+  w.nn = __shfl_sync(~0u, w.l_nn, l);
+}
+// The first sequence from the batch at w.base on; there is one while w.left > 0.
+__device__ __forceinline__ void walk_next_seq(const ApArgs &a, Walk &w, int lane) {
+  while (w.more == 0) {
+    w.base += 32;
+    walk_batch(a, w, lane);
+  }
+  walk_take_lane(w, __ffs(w.more) - 1);
+}
+
+__device__ __forceinline__ Walk walk_begin(const ApArgs &a, int me, int per_warp, int all,
+                                           int lane) {
+  Walk w = {};
+  w.me = me;
+  w.per_warp = per_warp;
+  int x = min((int64_t)me * per_warp, (int64_t)all);
+  w.left = min(per_warp, all - x);
+  if (w.left <= 0) return w;
+  const int pre = a.n_kv * a.p_tiles * a.p_stages;
+  int v = walk_batch(a, w, lane);
+  if (x < pre) {
+    w.b = -1;
+    w.st = a.p_stages;
+    w.tiles = a.p_tiles;
+    w.n_valid = a.n_shared;
+  } else {
+    x -= pre;
+    int l;
+    for (;;) {
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(~0u, v, d);
+        if (lane >= d) v += y;
+      }
+      const uint32_t past = __ballot_sync(~0u, x < v);
+      if (past) {
+        l = __ffs(past) - 1;
+        break;
+      }
+      x -= __shfl_sync(~0u, v, 31);
+      w.base += 32;
+      v = walk_batch(a, w, lane);
+    }
+    const int before = __shfl_sync(~0u, v, max(l - 1, 0));
+    if (l > 0) x -= before;
+    walk_take_lane(w, l);
+  }
+  const int group = x / w.st;
+  w.s0 = x - group * w.st;
+  w.kvh = group / w.tiles;
+  w.tile = group - w.kvh * w.tiles;
+  return w;
+}
+
+// The part of the next group that lies in the warp's stretch; w.left > 0.
+__device__ __forceinline__ Item walk_next(const ApArgs &a, Walk &w, int lane) {
+  Item it;
+  const int n = min(w.st - w.s0, w.left);
+  it.b = w.b;
+  it.nn = w.nn;
+  it.kvh = w.kvh;
+  it.r0 = w.tile * kRows;
+  it.n_valid = w.n_valid;
+  it.begins = w.s0 == 0;
+  it.ends = w.s0 + n == w.st;
+  it.shares = w.me << 16 | (w.st <= w.left ? 1 : 1 + (w.st - w.left + w.per_warp - 1) / w.per_warp);
+  it.k0 = w.s0 * kStageKeys;
+  it.k1 = it.k0 + n * kStageKeys;
+  if (it.b < 0) {
+    it.k1 = min(it.k1, a.n_shared);
+  } else {
+    it.k0 += a.n_shared;
+    // the last row of the tile sees furthest
+    const int t_last = min(quot(it.r0 + kRows - 1, a.by_g), w.nn - 1);
+    it.k1 = min(it.k1 + a.n_shared, it.n_valid - w.nn + t_last + 1);
+  }
+  w.left -= n;
+  w.s0 += n;
+  if (it.ends && w.left > 0) {
+    w.s0 = 0;
+    if (++w.tile == w.tiles) {
+      w.tile = 0;
+      if (++w.kvh == a.n_kv) {
+        w.kvh = 0;
+        walk_next_seq(a, w, lane);
+      }
+    }
+  }
+  return it;
+}
+
+// Row R of an item's; for the rows of one sequence nothing is read.
+__device__ __forceinline__ Row get_row(const ApArgs &a, const Item &it, int R) {
+  if (it.b < 0) return get_row(a, -1, it.kvh, R);
+  Row w;
+  const int t = quot(R, a.by_g);
+  w.h = it.kvh * a.g + (R - t * a.g);
+  w.m = t < it.nn ? it.b * a.T + t : -1;
+  w.end = t < it.nn ? it.n_valid - it.nn + t + 1 : 0;
+  return w;
+}
+
+__device__ __forceinline__ int item_stages(const Item &it) {
+  return it.k1 > it.k0 ? (it.k1 - it.k0 + kStageKeys - 1) / kStageKeys : 0;
 }
 
 }  // namespace
@@ -353,7 +465,7 @@ __device__ __forceinline__ void mma_stage(MmaState &w, uint32_t kb, uint32_t vb,
 __global__ void __launch_bounds__(kMmaWarps * 32, 1)
     attention_pages_mma_kernel(const __grid_constant__ CUtensorMap tmK,
                                const __grid_constant__ CUtensorMap tmV,
-                               const __grid_constant__ ApArgs a, int n_item) {
+                               const __grid_constant__ ApArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -369,75 +481,114 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
     }
   }
   __syncwarp();
+  // Behind the tensor-core kernel, which lets this one start once all its CTAs run (and what
+  // came before it is complete), there is nothing to wait for before the end: both only write
+  // parts of rows, and a CTA here starts as an SM is free.
   pdl_launch_dependents();
-  pdl_wait();
+  if (!a.behind) pdl_wait();
 
-  // neighbouring items (chunks of one row tile, heads of one sequence) on different SMs
-  const int step = gridDim.x * kMmaWarps;
-  const int first = warp * gridDim.x + blockIdx.x - 32 * step;
-  Cursor ld = {}, cp = {};
-  ld.base = cp.base = first;
-  cursor_next_item(a, ld, step, n_item, lane);
-  cp = ld;
+  // neighbouring stretches on different SMs: they share keys in L2, and few stages spread out
+  const int me = warp * gridDim.x + blockIdx.x;
+  const int all = all_stages(a, lane), unit = max(a.whole, 1);
+  const int warps = gridDim.x * kMmaWarps;
+  const int per_warp = max((all / unit + warps - 1) / warps, 1) * unit;
+  Walk walk = walk_begin(a, me, per_warp, all, lane);
 
-  // ---- loading: lane i < 2 * boxes brings one box (16 or 32 rows) of a stage ----
+  // ---- loading: lane i < 2 * boxes brings one box (16 to 64 rows) of a stage ----
   const int box = min(1 << a.page_shift, kStageKeys);
   const int boxes = kStageKeys / box;
   const bool act = lane < 2 * boxes, is_v = lane >= boxes;
   const int bx = is_v ? lane - boxes : lane;
+  Walk ahead = walk;  // of the loads
+  Item it;
+  int stage = 0, stages = 0;
+  auto next_item = [&]() {  // one with keys
+    stage = stages = 0;
+    while (stages == 0 && ahead.left > 0) {
+      it = walk_next(a, ahead, lane);
+      stages = item_stages(it);
+    }
+  };
   auto entry = [&]() -> int {  // page of this lane's box, n_pages: reads as zeros
-    const int pos = ld.it.k0 + ld.stage * kStageKeys + bx * box;
-    if (!act || ld.stages == 0 || pos >= ld.it.k1) return a.n_pages;
+    const int pos = it.k0 + stage * kStageKeys + bx * box;
+    if (!act || stages == 0 || pos >= it.k1) return a.n_pages;
     const int k = pos >> a.page_shift;
     int p = -1;
-    if (ld.it.b < 0) p = a.shared[k];
-    else if (k < a.max_pages) p = a.table[(int64_t)ld.it.b * a.max_pages + k];
+    if (it.b < 0) p = a.shared[k];
+    else if (k < a.max_pages) p = a.table[(int64_t)it.b * a.max_pages + k];
     if (p < 0 || p >= a.n_pages) {
       report_error(a.err, kErrEntry);
       p = a.n_pages;
     }
     return p;
   };
+  next_item();
   int page = entry();
   uint32_t loaded = 0;
   auto load = [&]() {
-    if (ld.stages == 0) return;
+    if (stages == 0) return;
     const int st = loaded % kStages;
     if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * kTileBytes);
     __syncwarp();
     if (act) {
-      const int pos = ld.it.k0 + ld.stage * kStageKeys + bx * box;
-      const int y = (ld.it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+      const int pos = it.k0 + stage * kStageKeys + bx * box;
+      const int y = (it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
       tma_load_3d(ring + (st * 2 + is_v) * kTileBytes + bx * box * 128, is_v ? &tmV : &tmK,
                   &full[st], 0, y, page);
     }
     ++loaded;
-    if (++ld.stage == ld.stages) cursor_next_item(a, ld, step, n_item, lane);
+    if (++stage == stages) next_item();
     page = entry();
   };
 #pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) load();
 
-  uint32_t n = 0;
-  while (cp.stages > 0) {
-    const Item &it = cp.it;
-    const Row row[2] = {get_row(a, it.b, it.kvh, it.r0 + (lane >> 2)),
-                        get_row(a, it.b, it.kvh, it.r0 + (lane >> 2) + 8)};
-    const bool hi = __any_sync(~0u, row[1].m >= 0);
-    MmaState w = {};
-    w.m[0] = w.m[1] = -INFINITY;
+  // an item with its rows and Q, which are fetched while the one before is worked on
+  struct Ready {
+    Item it;
+    Row row[2];
+    uint32_t q[4][4];
+  };
+  auto prepare = [&]() {
+    Ready y;
+    y.it = walk_next(a, walk, lane);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      if (row[r].m < 0) continue;
-      const uint32_t *src = reinterpret_cast<const uint32_t *>(a.Q + (int64_t)row[r].m * a.ldq +
-                                                               row[r].h * kPageHd) + (lane & 3);
+      y.row[r] = get_row(a, y.it, y.it.r0 + (lane >> 2) + 8 * r);
+      const Row &w = y.row[r];
+      const uint32_t *src = reinterpret_cast<const uint32_t *>(a.Q + (int64_t)w.m * a.ldq +
+                                                               w.h * kPageHd) + (lane & 3);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        w.q[ks][r] = src[ks * 8];
-        w.q[ks][r + 2] = src[ks * 8 + 4];
+        y.q[ks][r] = w.m < 0 ? 0u : src[ks * 8];
+        y.q[ks][r + 2] = w.m < 0 ? 0u : src[ks * 8 + 4];
       }
     }
-    for (int s = 0; s < cp.stages; ++s, ++n) {
+    return y;
+  };
+  uint32_t n = 0;
+  bool more = walk.left > 0;
+  Ready ready;
+  if (more) ready = prepare();
+  while (more) {
+    const Ready cur = ready;
+    const Item &it = cur.it;
+    const Row(&row)[2] = cur.row;
+    more = walk.left > 0;
+    if (more) ready = prepare();
+    const int stages = item_stages(it);
+    const bool hi = __any_sync(~0u, row[1].m >= 0);
+    MmaState w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w.q[i][k] = cur.q[i][k];
+        w.o[i][k] = w.o[i + 4][k] = 0.0f;
+      }
+    w.m[0] = w.m[1] = -INFINITY;
+    w.l[0] = w.l[1] = 0.0f;
+    for (int s = 0; s < stages; ++s, ++n) {
       load();  // into the stage that was read last
       const int st = n % kStages;
       if (!__all_sync(~0u, mbar_wait(&full[st], (n / kStages) & 1, nullptr, a.err, kErrWaitFull))) {
@@ -474,15 +625,19 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
         for (int d = 0; d < 8; ++d)
           dst[4 * d] = pack_bf2(w.o[d][2 * r] * inv, w.o[d][2 * r + 1] * inv);
       } else {
-        const int64_t at = it.slot * a.rows + (int64_t)row[r].m * (a.n_kv * a.g) + row[r].h;
+        const int64_t id = (int64_t)row[r].m * (a.n_kv * a.g) + row[r].h;
+        if (it.begins && (lane & 3) == 0) a.shares[(it.b < 0 ? 0 : a.rows) + id] = it.shares;
+        const int64_t at = it.begins && it.ends
+                               ? (it.b < 0 ? 0 : a.slots - 1) * a.rows + id
+                               : a.slots * a.rows + (me * 2 + it.begins) * kRows + (lane >> 2) + 8 * r;
         float2 *dst = reinterpret_cast<float2 *>(a.Op + at * kPageHd + (lane & 3) * 2);
 #pragma unroll
         for (int d = 0; d < 8; ++d) dst[4 * d] = make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
         if ((lane & 3) == 0) a.ml[at] = make_float2(w.m[r] * kScale2, l);
       }
     }
-    cursor_next_item(a, cp, step, n_item, lane);
   }
+  if (a.behind) pdl_wait();  // this kernel's end is to mean the other's too
 }
 
 // ---------------------------------------------------------------------------
@@ -553,13 +708,13 @@ __device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx) {
     it.k1 = min(it.k0 + a.p_chunk, end);
     return it;
   }
-  const int full = a.pairs * a.full_splits;
+  const int full = a.pairs * a.p_splits;
   it.b = -1;
   it.kvh = idx / (full + a.one_splits);
   const int q = idx - it.kvh * (full + a.one_splits);
   const bool one = q >= full;
-  const int pair = one ? a.pairs : q / a.full_splits;
-  it.slot = one ? q - full : q - pair * a.full_splits;
+  const int pair = one ? a.pairs : q / a.p_splits;
+  it.slot = one ? q - full : q - pair * a.p_splits;
   it.r0 = pair * kPairRows;
   it.r1 = min(it.r0 + kPairRows, a.n_seq * a.T * a.g);
   const int chunk = one ? a.one_chunk : a.p_chunk;
@@ -590,8 +745,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t *sKV = smem + 2 * kTcTile;        // [stages] K, V
   TcCtl *ctl = reinterpret_cast<TcCtl *>(sKV + kTcStages * 2 * kTcTile);
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // (after the wait: see attention_pages_mma_kernel)
   const TcItem it = get_tc_item(a, blockIdx.x);
   const int n_rows = it.r1 - it.r0;
   const int blocks = it.k1 > it.k0 ? (it.k1 - it.k0 + kTcKeys - 1) / kTcKeys : 0;
@@ -698,9 +853,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       float mx[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
+        mx[c] = max3(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]), -INFINITY);
 #pragma unroll
-        for (int k = 1; k < 32; ++k) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][k]));
+        for (int k = 2; k < 32; k += 2)
+          mx[c] = max3(mx[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool up = grown(top, m);
@@ -733,16 +889,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       // Weights, 32 keys at a time: the exponentials of a chunk are issued between the scaling of
       // the next chunk and the sums and packing of the last, whose results have arrived by then
-      // (a warp issues in order and would otherwise wait for each).
-      float sum[4] = {};
-      auto scale = [&](int c, int k) {
-        s[c][k] = __float_as_uint(fmaf(__uint_as_float(s[c][k]), kScale2, -ms));
+      // (a warp issues in order and would otherwise wait for each). Scaling and sums work on
+      // pairs (f32x2).
+      const F2 scale2 = f2(kScale2, kScale2), minus = f2(-ms, -ms);
+      F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+      auto pair = [&](int c, int k) {
+        return f2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       };
+      auto put = [&](int c, int k, F2 v) {
+        float x, y;
+        f2_split(v, x, y);
+        s[c][k] = __float_as_uint(x);
+        s[c][k + 1] = __float_as_uint(y);
+      };
+      auto scale = [&](int c, int k) { put(c, k, f2_fma(pair(c, k), scale2, minus)); };
       auto take = [&](int c, int k) {  // keys k, k + 1
-        const float x = __uint_as_float(s[c][k]), y = __uint_as_float(s[c][k + 1]);
-        sum[k & 2] += x;
-        sum[(k & 2) + 1] += y;
-        s[c][k / 2] = pack_bf2(x, y);
+        sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], pair(c, k));
+        s[c][k / 2] = pack_bf2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       };
       auto store = [&](int c) {  // chunks c - 1 and c
         uint32_t p[32];
@@ -754,17 +917,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_st_32x32b_x32(trow + kColP + 16 * (c - 1), p);
       };
 #pragma unroll
-      for (int k = 0; k < 32; ++k) scale(0, k);
+      for (int k = 0; k < 32; k += 2) scale(0, k);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           s[c][k] = __float_as_uint(ex2(__uint_as_float(s[c][k])));
           s[c][k + 1] = __float_as_uint(ex2(__uint_as_float(s[c][k + 1])));
-          if (c < 3) {
-            scale(c + 1, k);
-            scale(c + 1, k + 1);
-          }
+          if (c < 3) scale(c + 1, k);
           if (c > 0) take(c - 1, k);
         }
         if (c == 2) store(1);
@@ -773,7 +933,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int k = 0; k < 32; k += 2) take(3, k);
       store(3);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      {
+        float x, y;
+        f2_split(f2_add(sum[0], sum[1]), x, y);
+        l += x + y;
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -954,9 +1118,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// The join of a row's items, a warp a row: a lane a slot for the weights, then
-// two dims a lane, eight slots' loads in flight. An item without keys below the
-// row's end was not run: its slot counts as weight zero, unread.
+// The join of a row's parts, a warp a row: a lane a part for the weights, then
+// two dims a lane, eight parts' loads in flight.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
     attention_pages_join_kernel(const __grid_constant__ ApArgs a) {
@@ -970,45 +1133,58 @@ __global__ void __launch_bounds__(256)
   const int nn = seq_new(a, b);
   if (t >= nn) return;
   const int end = seq_len(a, b) - nn + t + 1;
-  const int slots = a.p_splits + a.t_splits;
-  // the row's place among the prefix rows of its key head tells its items' chunk
-  const int R = m * a.g + (h - quot(h, a.by_g) * a.g);
-  const int p_chunk = a.one_splits && R >= a.pairs * kPairRows ? a.one_chunk : a.p_chunk;
+  // parts: tensor-core items over the prefix, the group over the prefix, the group over the tail
+  const int gi = h - quot(h, a.by_g) * a.g;
+  const int R = m * a.g + gi, Rt = t * a.g + gi;  // among the rows of the key head: all, b's
+  int n0 = 0, pre = 0, tail = 0;
+  if (a.p_splits) {
+    const int chunk = a.one_splits && R >= a.pairs * kPairRows ? a.one_chunk : a.p_chunk;
+    n0 = (min(max(end, 0), a.p_end) + chunk - 1) / chunk;
+  }
+  if (a.p_stages) pre = a.shares[row];
+  if (!a.by_seq && tail_stages(a, seq_len(a, b)) > 0) tail = a.shares[a.rows + row];
+  const int n1 = n0 + (pre & 0xffff), n2 = n1 + (tail & 0xffff);
+  auto part = [&](int i) -> int64_t {
+    if (i < n0) return i * a.rows + row;
+    const bool of_tail = i >= n1;
+    const int sh = of_tail ? tail : pre, k = i - (of_tail ? n1 : n0);
+    if ((sh & 0xffff) == 1) return (of_tail ? a.slots - 1 : 0) * a.rows + row;
+    return a.slots * a.rows + (((sh >> 16) + k) * 2 + (k == 0)) * kRows +
+           ((of_tail ? Rt : R) & (kRows - 1));
+  };
   float mx = -INFINITY, l = 0.0f;
   float2 acc = make_float2(0.0f, 0.0f);
-  for (int base = 0; base < slots; base += 32) {
-    const int s = base + lane;
-    const bool live = s < a.p_splits ? (int64_t)s * p_chunk < min(end, a.p_end)
-                                     : s < slots && a.n_shared + (int64_t)(s - a.p_splits) *
-                                                                     a.t_chunk < end;
-    const float2 v = live ? a.ml[s * a.rows + row] : make_float2(-INFINITY, 0.0f);
+  for (int base = 0; base < n2; base += 32) {
+    const bool live = base + lane < n2;
+    const int64_t at = live ? part(base + lane) : 0;
+    const float2 v = live ? a.ml[at] : make_float2(-INFINITY, 0.0f);
     float top = v.x;
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     top = fmaxf(top, mx);
     const float ms = safe_max(top), f = ex2(mx - ms), w = live ? ex2(v.x - ms) : 0.0f;
     mx = top;
-    l = l * f + w * v.y;  // this lane's slots
+    l = l * f + w * v.y;  // this lane's parts
     acc.x *= f;
     acc.y *= f;
-    for (uint32_t todo = __ballot_sync(~0u, live); todo;) {
+    const int n = min(32, n2 - base);
+    for (int k0 = 0; k0 < n; k0 += 8) {
       float2 x[8];
       float wx[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int k = todo ? __ffs(todo) - 1 : 0;
-        wx[i] = __shfl_sync(~0u, w, k);
-        if (!todo) wx[i] = 0.0f;
-        x[i] = todo ? reinterpret_cast<const float2 *>(
-                          a.Op + ((base + k) * a.rows + row) * kPageHd)[lane]
-                    : make_float2(0.0f, 0.0f);
-        todo &= todo - 1;
+        const int k = k0 + i;
+        wx[i] = __shfl_sync(~0u, w, k & 31);
+        const int64_t from = __shfl_sync(~0u, at, k & 31);
+        x[i] = k < n ? reinterpret_cast<const float2 *>(a.Op + from * kPageHd)[lane]
+                     : make_float2(0.0f, 0.0f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        acc.x += wx[i] * x[i].x;
-        acc.y += wx[i] * x[i].y;
-      }
+      for (int i = 0; i < 8; ++i)
+        if (k0 + i < n) {
+          acc.x += wx[i] * x[i].x;
+          acc.y += wx[i] * x[i].y;
+        }
     }
   }
 #pragma unroll
@@ -1024,11 +1200,14 @@ __global__ void __launch_bounds__(256)
 namespace {
 
 struct Plan {
-  bool tc;         // a tensor-core launch
-  bool by_seq;     // it covers everything
-  int tc_items;
-  int p_tiles, p_splits, p_chunk, t_tiles, t_splits, t_chunk;
-  int pairs, full_splits, one_splits, one_chunk, p_end;
+  int tc_items;    // of the tensor-core kernel, 0: not launched
+  bool by_seq;     // they cover everything
+  int pairs, p_splits, p_chunk, one_splits, one_chunk, p_end;
+  int grid;        // of the 16-row kernel, 0: not launched
+  int p_tiles, p_stages, whole;
+  bool direct;
+  int slots;
+  size_t parts;    // of rows in the workspace
 };
 
 int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -1041,25 +1220,35 @@ int chunk_keys(int64_t keys, int64_t groups, int64_t want, int min_keys, int ste
   return (int)(c < min_keys ? min_keys : c);
 }
 
-Plan make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared) {
+// W8A8_ERR_UNSUPPORTED: more stages than 32 bits count.
+int make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared, Plan *out) {
   Plan p = {};
   const int g = n_head / n_kv;
-  const int64_t want = kSms * kMmaWarps * 3;  // 16-row items: some for every warp
   const int64_t own = (int64_t)T * g, all = own * n_seq;  // rows of a key head
+  const int64_t rows = all * n_kv;
   p.p_end = n_shared;
   if (own >= 64) {
     // enough rows a sequence to fill a tile: prefix and tail in one item
-    p.tc = p.by_seq = true;
+    p.by_seq = true;
     p.pairs = (int)cdiv(own, kPairRows);
     const int64_t groups = (int64_t)n_seq * n_kv * p.pairs;
     p.p_chunk = chunk_keys(max_ctx, groups, groups >= kSms ? groups : kSms, 4 * kTcKeys, kTcKeys);
     p.p_splits = (int)cdiv(max_ctx, p.p_chunk);
     p.p_end = max_ctx;
+    if (groups * p.p_splits > 0x7fffffff) return W8A8_ERR_UNSUPPORTED;
     p.tc_items = (int)(groups * p.p_splits);
-    return p;
+    p.slots = p.p_splits;
+    p.direct = p.slots == 1;
+    p.parts = p.direct ? 0 : (size_t)rows * p.slots;
+    *out = p;
+    return W8A8_OK;
   }
-  if (n_shared > 0 && all > 32) {
-    p.tc = true;
+  const int64_t p_stages = cdiv(n_shared, kStageKeys), p_tiles = cdiv(all, kRows);
+  const int tail = max_ctx - n_shared > 0 ? max_ctx - n_shared : 1;
+  const int64_t t_stages = cdiv(tail, kStageKeys), t_tiles = cdiv(own, kRows);
+  int64_t stages = n_seq * t_tiles * t_stages * n_kv;
+  const int64_t pre = n_kv * p_tiles * p_stages;
+  if (pre > kMinTcStages && all > kRows) {
     // full pairs get twice the chunks of a last single tile, whose blocks take half the time;
     // one CTA an SM in all, if there are that few
     const int64_t tiles = cdiv(all, kTileRows);
@@ -1072,20 +1261,28 @@ Plan make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared
     if (s2 < 1) s2 = 1;
     p.p_chunk = chunk_keys(n_shared, 1, s2, 2 * kTcKeys, kTcKeys);
     p.one_chunk = chunk_keys(n_shared, 1, s1, 2 * kTcKeys, kTcKeys);
-    p.full_splits = p.pairs ? (int)cdiv(n_shared, p.p_chunk) : 0;
+    p.p_splits = (int)cdiv(n_shared, p.pairs ? p.p_chunk : p.one_chunk);
     p.one_splits = single ? (int)cdiv(n_shared, p.one_chunk) : 0;
-    p.p_splits = p.full_splits > p.one_splits ? p.full_splits : p.one_splits;
-    p.tc_items = n_kv * (p.pairs * p.full_splits + p.one_splits);
+    p.tc_items = n_kv * (p.pairs * p.p_splits + p.one_splits);
+    p.slots = p.p_splits > p.one_splits ? p.p_splits : p.one_splits;
   } else if (n_shared > 0) {
-    p.p_tiles = (int)cdiv(all, kRows);
-    p.p_chunk = chunk_keys(n_shared, (int64_t)n_kv * p.p_tiles, want, 2 * kStageKeys, kStageKeys);
-    p.p_splits = (int)cdiv(n_shared, p.p_chunk);
+    p.p_tiles = (int)p_tiles;
+    p.p_stages = (int)p_stages;
+    stages += pre;
+    p.slots = 1;
+  } else if (t_stages <= 4) {
+    // short sequences, nothing shared: whole groups, and no join
+    p.whole = (int)t_stages;
+    p.direct = true;
   }
-  p.t_tiles = (int)cdiv(own, kRows);
-  const int tail = max_ctx - n_shared > 0 ? max_ctx - n_shared : 1;
-  p.t_chunk = chunk_keys(tail, (int64_t)n_seq * n_kv * p.t_tiles, want, 2 * kStageKeys, kStageKeys);
-  p.t_splits = (int)cdiv(tail, p.t_chunk);
-  return p;
+  if (stages > 0x7fffffff - kSms * kMmaWarps) return W8A8_ERR_UNSUPPORTED;
+  const int64_t work = p.whole ? stages / p.whole : stages;
+  p.grid = (int)(work < kSms ? work : kSms);
+  p.slots += 1;
+  const int64_t warps = work < kSms * kMmaWarps ? work : kSms * kMmaWarps;  // with a stretch
+  p.parts = p.direct ? 0 : (size_t)(rows * p.slots + warps * 2 * kRows);
+  *out = p;
+  return W8A8_OK;
 }
 
 // Shared-memory opt-in of a kernel on the current device, once.
@@ -1105,18 +1302,21 @@ int opt_in_smem(K *kernel, size_t bytes, bool (&done)[64]) {
 
 }  // namespace
 
+// Parts of rows (64 sums, a maximum and a sum of weights each), and two words a row.
 size_t attention_pages_workspace_bytes(int n_seq, int T, int n_head, int n_kv, int max_ctx,
                                        int n_shared) {
-  const Plan p = make_plan(n_seq, T, n_head, n_kv, max_ctx, n_shared);
-  const int slots = p.p_splits + p.t_splits;
-  const size_t rows = (size_t)n_seq * T * n_head;
-  return slots <= 1 ? 16 : slots * rows * (kPageHd * sizeof(float) + sizeof(float2));
+  Plan p;
+  if (make_plan(n_seq, T, n_head, n_kv, max_ctx, n_shared, &p)) return 0;
+  if (p.direct) return 16;
+  return p.parts * (kPageHd * sizeof(float) + sizeof(float2)) +
+         2 * sizeof(int) * (size_t)n_seq * T * n_head;
 }
 
-int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_count,
-                           cudaStream_t s) {
+int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStream_t s) {
   const int g = q.n_head / c.n_kv_head;
-  const Plan p = make_plan(q.n_seq, q.T, q.n_head, c.n_kv_head, q.max_ctx, q.n_shared);
+  Plan p;
+  int st = make_plan(q.n_seq, q.T, q.n_head, c.n_kv_head, q.max_ctx, q.n_shared, &p);
+  if (st) return st;
   ApArgs a = {};
   a.Q = q.Q;
   a.ldq = q.ldq;
@@ -1136,30 +1336,25 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_co
   a.max_ctx = q.max_ctx;
   a.n_shared = q.n_shared;
   a.p_tiles = p.p_tiles;
-  a.p_splits = p.p_splits;
-  a.p_chunk = p.p_chunk;
-  a.t_tiles = p.t_tiles;
-  a.t_splits = p.t_splits;
-  a.t_chunk = p.t_chunk;
+  a.p_stages = p.p_stages;
+  a.whole = p.whole;
   a.by_seq = p.by_seq;
   a.pairs = p.pairs;
-  a.full_splits = p.full_splits;
+  a.p_splits = p.p_splits;
+  a.p_chunk = p.p_chunk;
   a.one_splits = p.one_splits;
   a.one_chunk = p.one_chunk;
   a.p_end = p.p_end;
+  a.direct = p.direct;
+  a.behind = p.tc_items > 0 && p.grid > 0;
   a.rows = (int64_t)q.n_seq * q.T * q.n_head;
   a.by_g = make_div(g);
   a.by_T = make_div(q.T);
-  a.by_kv = make_div(c.n_kv_head);
   a.by_head = make_div(q.n_head);
-  a.by_seq_n = make_div(q.n_seq);
-  a.by_pt = make_div(p.p_tiles);
-  a.by_tt = make_div(p.t_tiles);
-  const int slots = p.p_splits + p.t_splits;
-  a.direct = slots == 1;
+  a.slots = p.slots;
   a.Op = reinterpret_cast<float *>(q.ws);
-  a.ml = reinterpret_cast<float2 *>(a.Op + (size_t)slots * a.rows * kPageHd);
-  int st;
+  a.ml = reinterpret_cast<float2 *>(a.Op + p.parts * kPageHd);
+  a.shares = reinterpret_cast<int *>(a.ml + p.parts);
   DeviceCtx *ctx = device_ctx(&st);
   if (!ctx) return st;
   a.err = ctx->err;
@@ -1175,7 +1370,7 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_co
                                 kPageHd * 2, (uint64_t)c.page_stride * 2, kPageHd, box);
   };
   static bool tc_ready[64], mma_ready[64];
-  if (p.tc) {
+  if (p.tc_items) {
     const size_t smem = 1024 + (2 + 2 * kTcStages) * kTcTile + sizeof(TcCtl);
     st = opt_in_smem(attention_pages_tc_kernel, smem, tc_ready);
     if (st || (st = maps(kBoxRows))) return st;
@@ -1184,15 +1379,11 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, int sm_co
     st = check_launch("attention_pages_tc");
     if (st) return st;
   }
-  const int64_t items = (int64_t)a.n_kv * p.p_tiles * p.p_splits +
-                        (int64_t)a.n_seq * a.n_kv * p.t_tiles * p.t_splits;
-  if (items > 0) {
+  if (p.grid) {
     const size_t smem = 1024 + kMmaWarps * kStages * 2 * kTileBytes + sizeof(MmaSmem);
     st = opt_in_smem(attention_pages_mma_kernel, smem, mma_ready);
     if (st || (st = maps(kStageKeys))) return st;
-    const int64_t grid = items < sm_count ? items : sm_count;
-    launch_pdl(attention_pages_mma_kernel, dim3((unsigned)grid), dim3(kMmaWarps * 32), smem, s,
-               tmK, tmV, a, (int)items);
+    launch_pdl(attention_pages_mma_kernel, dim3(p.grid), dim3(kMmaWarps * 32), smem, s, tmK, tmV, a);
     st = check_launch("attention_pages_mma");
     if (st) return st;
   }

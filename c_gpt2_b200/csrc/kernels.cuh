@@ -242,7 +242,6 @@ struct AttnPagesCall {
 };
 size_t attention_pages_workspace_bytes(int n_seq, int T, int n_head, int n_kv_head, int max_ctx,
                                        int n_shared);
-int launch_attention_pages(const PagesArgs &a, const AttnPagesCall &c, int sm_count,
-                           cudaStream_t s);
+int launch_attention_pages(const PagesArgs &a, const AttnPagesCall &c, cudaStream_t s);
 
 }  // namespace w8a8
