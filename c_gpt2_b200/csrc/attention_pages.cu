@@ -70,23 +70,24 @@ struct ApArgs {
   // sequence [n_kv][its row tiles] over its tail (see Walk)
   int p_tiles, p_stages;
   int whole;           // stages given to every sequence's groups, none split; 0: as many as it has
-  // tensor-core items (see attention_pages_tc_kernel)
-  int by_seq;          // rows of one sequence over all its keys, or of all over the prefix
-  int pairs;           // pairs of 128-row tiles: of a sequence, or full ones of all rows
-  int p_splits, p_chunk;      // items and keys of an item; of the prefix of a full pair
-  int one_splits, one_chunk;  // those of a last single tile
-  int p_end;           // these items cover positions below this
+  // tensor-core items: rows of one sequence over all its keys, [pairs][n_seq][n_kv][splits]
+  // of `chunk` keys; or of all sequences over the prefix, per_kv CTAs a key head (see
+  // plan_across)
+  int by_seq, pairs, splits, chunk, per_kv;
+  int tc;              // the tensor-core kernel runs
   int behind;          // the 16-row kernel runs behind the tensor-core kernel
   int direct;          // every row is one item's or group's, which writes O itself
   int64_t rows;        // n_seq * T * n_head
   Div by_g, by_T, by_head;
-  // Parts of rows: [slots][rows], one for each tensor-core item over a row's prefix, or one for
-  // its 16-row group over it; one for its group over the tail; then [warps][2][16], of groups
-  // that several warps share: a warp's rows of the group it joined, and of the one it began.
-  int slots;
+  // Parts of rows: 256 of each tensor-core item; then, of the 16-row groups, one a row over the
+  // prefix (at part_p) and one over the tail (part_t); and, of groups that several warps share,
+  // [warps][2][16] (part_f): a warp's rows of the group it joined, and of the one it began.
+  int64_t part_p, part_t, part_f;
   float *Op;           // [part][64]
   float2 *ml;          // [part] maximum (base 2), sum
-  int *shares;         // [prefix, tail][rows] first warp of the row's group * 2^16 + warps
+  // [3][rows]: first part (tensor-core items) or first warp of the row's parts over the prefix,
+  // their number, and for the tail first warp * 2^16 + number
+  int *shares;
   int *err;
 };
 
@@ -196,7 +197,7 @@ struct Item {
   int kvh, r0;  // key head; first row of the tile among the (m, g) rows of b or of all
   int k0, k1;   // positions
   int n_valid;  // positions that hold anything
-  int shares;   // where `begins`: first warp of the group * 2^16 + its warps
+  int warps;    // where `begins`: warps that share the group
   bool begins, ends;
 };
 
@@ -316,7 +317,7 @@ __device__ __forceinline__ Item walk_next(const ApArgs &a, Walk &w, int lane) {
   it.n_valid = w.n_valid;
   it.begins = w.s0 == 0;
   it.ends = w.s0 + n == w.st;
-  it.shares = w.me << 16 | (w.st <= w.left ? 1 : 1 + (w.st - w.left + w.per_warp - 1) / w.per_warp);
+  it.warps = w.st <= w.left ? 1 : 1 + (w.st - w.left + w.per_warp - 1) / w.per_warp;
   it.k0 = w.s0 * kStageKeys;
   it.k1 = it.k0 + n * kStageKeys;
   if (it.b < 0) {
@@ -626,10 +627,17 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
           dst[4 * d] = pack_bf2(w.o[d][2 * r] * inv, w.o[d][2 * r + 1] * inv);
       } else {
         const int64_t id = (int64_t)row[r].m * (a.n_kv * a.g) + row[r].h;
-        if (it.begins && (lane & 3) == 0) a.shares[(it.b < 0 ? 0 : a.rows) + id] = it.shares;
+        if (it.begins && (lane & 3) == 0) {
+          if (it.b < 0) {
+            a.shares[id] = me;
+            a.shares[a.rows + id] = it.warps;
+          } else {
+            a.shares[2 * a.rows + id] = me << 16 | it.warps;
+          }
+        }
         const int64_t at = it.begins && it.ends
-                               ? (it.b < 0 ? 0 : a.slots - 1) * a.rows + id
-                               : a.slots * a.rows + (me * 2 + it.begins) * kRows + (lane >> 2) + 8 * r;
+                               ? (it.b < 0 ? a.part_p : a.part_t) + id
+                               : a.part_f + (me * 2 + it.begins) * kRows + (lane >> 2) + 8 * r;
         float2 *dst = reinterpret_cast<float2 *>(a.Op + at * kPageHd + (lane & 3) * 2);
 #pragma unroll
         for (int d = 0; d < 8; ++d) dst[4 * d] = make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
@@ -684,51 +692,136 @@ struct TcCtl {
 
 struct TcItem {
   int b, kvh;      // sequence, -1: rows of all
-  int r0, r1;      // rows among the (m, g) rows of b, or of all
-  int slot, k0, k1, n_valid;
+  int r0, r1;      // rows among the (m, g) rows of b, or of all that hold a query
+  int k0, k1, n_valid;
+  int split, splits;  // of the rows' items over their keys
 };
 
-__device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx) {
+// The prefix items of a key head: the rows that hold a query, packed (their number is known
+// here only), in pairs of tiles and perhaps a last single one. A CTA's time goes by its
+// blocks, and a single tile's take half as long, so its items get twice the keys; one CTA an
+// SM in all if the rows are few.
+struct Across {
+  int rows, pairs, s2, c2, s1, c1;  // s1 = 0: no single tile
+};
+__device__ __forceinline__ Across plan_across(const ApArgs &a, int lane) {
+  Across p;
+  int valid = a.n_seq * a.T;
+  if (a.n_new) {
+    valid = 0;
+#pragma unroll 4
+    for (int b = lane; b < a.n_seq; b += 32) valid += seq_new(a, b);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) valid += __shfl_xor_sync(~0u, valid, d);
+  }
+  p.rows = valid * a.g;
+  const int tiles = (p.rows + kTileRows - 1) / kTileRows, single = tiles & 1;
+  p.pairs = tiles >> 1;
+  auto chunk = [&](int splits) {
+    const int c = ((a.n_shared + splits - 1) / splits + kTcKeys - 1) / kTcKeys * kTcKeys;
+    return max(c, 2 * kTcKeys);
+  };
+  p.s1 = p.s2 = 0;
+  p.c1 = p.c2 = kTcKeys;
+  if (tiles == 0) return p;
+  const int s1 = max(1, a.per_kv / tiles);
+  if (single) {
+    p.c1 = chunk(s1);
+    p.s1 = (a.n_shared + p.c1 - 1) / p.c1;
+  }
+  if (p.pairs) {
+    p.c2 = chunk(max(1, (a.per_kv - s1 * single) / p.pairs));
+    p.s2 = (a.n_shared + p.c2 - 1) / p.c2;
+  }
+  return p;
+}
+
+__device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx, int lane) {
   TcItem it;
+  it.split = 0;
   if (a.by_seq) {
     // the last rows of a sequence see furthest: those items first
-    const int s = idx % a.p_splits;
-    int q = idx / a.p_splits;
+    int q = idx / a.splits;
+    it.split = idx - q * a.splits;
     it.kvh = q % a.n_kv;
     q /= a.n_kv;
     it.b = q % a.n_seq;
     const int pair = a.pairs - 1 - q / a.n_seq;
-    const int nn = seq_new(a, it.b), n = seq_len(a, it.b);
+    const int nn = seq_new(a, it.b);
+    it.n_valid = seq_len(a, it.b);
     it.r0 = pair * kPairRows;
     it.r1 = min(it.r0 + kPairRows, nn * a.g);
-    it.slot = s;
-    it.k0 = s * a.p_chunk;
-    it.n_valid = n;
-    const int end = it.r1 > it.r0 ? n - nn + (it.r1 - 1) / a.g + 1 : 0;
-    it.k1 = min(it.k0 + a.p_chunk, end);
+    const int end = it.r1 > it.r0 ? max(it.n_valid - nn + (it.r1 - 1) / a.g + 1, 0) : 0;
+    it.splits = (end + a.chunk - 1) / a.chunk;
+    it.k0 = it.split * a.chunk;
+    it.k1 = min(it.k0 + a.chunk, end);
     return it;
   }
-  const int full = a.pairs * a.p_splits;
+  const Across p = plan_across(a, lane);
+  const int full = p.pairs * p.s2, each = full + p.s1;
   it.b = -1;
-  it.kvh = idx / (full + a.one_splits);
-  const int q = idx - it.kvh * (full + a.one_splits);
-  const bool one = q >= full;
-  const int pair = one ? a.pairs : q / a.p_splits;
-  it.slot = one ? q - full : q - pair * a.p_splits;
-  it.r0 = pair * kPairRows;
-  it.r1 = min(it.r0 + kPairRows, a.n_seq * a.T * a.g);
-  const int chunk = one ? a.one_chunk : a.p_chunk;
-  it.k0 = it.slot * chunk;
-  it.k1 = min(it.k0 + chunk, a.n_shared);
+  it.kvh = each ? idx / each : a.n_kv;
+  it.r0 = it.r1 = it.k0 = it.k1 = it.splits = 0;
   it.n_valid = a.n_shared;
+  if (it.kvh >= a.n_kv) return it;  // one CTA too many
+  const int q = idx - it.kvh * each;
+  const bool one = q >= full;
+  const int pair = one ? p.pairs : q / p.s2;
+  const int chunk = one ? p.c1 : p.c2;
+  it.split = one ? q - full : q - pair * p.s2;
+  it.splits = one ? p.s1 : p.s2;
+  it.r0 = pair * kPairRows;
+  it.r1 = min(it.r0 + kPairRows, p.rows);
+  it.k0 = it.split * chunk;
+  it.k1 = min(it.k0 + chunk, a.n_shared);
   return it;
 }
 
-__device__ __forceinline__ Row get_tc_row(const ApArgs &a, const TcItem &it, int R) {
-  Row w = get_row(a, it.b, it.kvh, R);
-  if (R >= it.r1) {
-    w.m = -1;
-    w.end = 0;
+// Row R of the item, for a lane of a converged warp. Among the packed rows of a padded batch the
+// sequence is searched for, 32 at a time.
+__device__ __forceinline__ Row get_tc_row(const ApArgs &a, const TcItem &it, int R, int lane) {
+  Row w;
+  w.m = -1;
+  w.h = w.end = 0;
+  const int j = quot(R, a.by_g);  // query among it.b's, or among all
+  int b = it.b, t = j;
+  if (b < 0 && !a.n_new) {
+    b = quot(j, a.by_T);
+    t = j - b * a.T;
+  } else if (b < 0) {
+    int start = 0;
+    for (int base = 0; base < a.n_seq; base += 32) {
+      int upto = base + lane < a.n_seq ? seq_new(a, base + lane) : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(~0u, upto, d);
+        if (lane >= d) upto += y;
+      }
+      const int in = __shfl_sync(~0u, upto, 31);
+      const bool mine = j >= start && j < start + in;
+      if (__any_sync(~0u, mine)) {
+        int l = 0, before = 0;  // lanes whose sequences end at or before j
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+          const int y = __shfl_sync(~0u, upto, l + d - 1);
+          if (y <= j - start) {
+            l += d;
+            before = y;
+          }
+        }
+        if (mine) {
+          b = base + l;
+          t = j - start - before;
+        }
+      }
+      start += in;
+      if (__all_sync(~0u, j < start || R >= it.r1)) break;
+    }
+  }
+  if (R < it.r1) {
+    w.h = it.kvh * a.g + (R - j * a.g);
+    w.m = b * a.T + t;
+    w.end = seq_len(a, b) - seq_new(a, b) + t + 1;
   }
   return w;
 }
@@ -747,12 +840,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();  // (after the wait: see attention_pages_mma_kernel)
-  const TcItem it = get_tc_item(a, blockIdx.x);
+  const TcItem it = get_tc_item(a, blockIdx.x, lane);
   const int n_rows = it.r1 - it.r0;
   const int blocks = it.k1 > it.k0 ? (it.k1 - it.k0 + kTcKeys - 1) / kTcKeys : 0;
-  // an item without keys: its slot is not read, unless rows get their zeros here
-  if (n_rows <= 0 || (blocks == 0 && !a.direct)) return;
+  if (n_rows <= 0) return;
   const bool one = n_rows <= kTileRows;      // both groups on one tile
+  // an item without keys leaves no part, unless rows get their zeros here
+  if (blocks == 0 && !a.direct && it.split > 0) return;
   const int units = one ? blocks : 2 * blocks;  // unit u: group u & 1
   // the last block reaches behind the positions that hold anything
   const bool v_cut = it.k0 + blocks * kTcKeys > it.n_valid;
@@ -791,7 +885,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---------------- softmax ----------------
     const int g = warp >> 2, qd = warp & 3;
     const int r = qd * 32 + lane;  // TMEM lane
-    const Row row = get_tc_row(a, it, it.r0 + (one ? 0 : g) * kTileRows + r);
+    const Row row = get_tc_row(a, it, it.r0 + (one ? 0 : g) * kTileRows + r, lane);
     const bool idle = __all_sync(~0u, row.m < 0);  // no rows in this warp
     const uint32_t trow = tmem + g * kColGroup + ((uint32_t)(qd * 32) << 16);
     // Q row into its swizzled place
@@ -967,7 +1061,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l_all = f0 * l + f1 * w.y;
       }
       const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
-      const int64_t at = it.slot * a.rows + (int64_t)row.m * (a.n_kv * a.g) + row.h;
+      const int at = blockIdx.x * kPairRows + g * kTileRows + r;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t o[16], o1[16];
@@ -992,14 +1086,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) dst[k] = pack_bf2(x[2 * k] * inv, x[2 * k + 1] * inv);
           } else {
-            float4 *dst = reinterpret_cast<float4 *>(a.Op + at * kPageHd + 16 * c);
+            float4 *dst = reinterpret_cast<float4 *>(a.Op + (int64_t)at * kPageHd + 16 * c);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               dst[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
           }
         }
       }
-      if (row.m >= 0 && !a.direct) a.ml[at] = make_float2(m_all, l_all);
+      if (row.m >= 0 && !a.direct) {
+        a.ml[at] = make_float2(m_all, l_all);
+        if (it.split == 0) {
+          const int64_t id = (int64_t)row.m * (a.n_kv * a.g) + row.h;
+          a.shares[id] = at;
+          a.shares[a.rows + id] = it.splits;
+        }
+      }
     }
   } else {
     reg_dealloc<88>();
@@ -1132,25 +1233,23 @@ __global__ void __launch_bounds__(256)
   const int b = quot(m, a.by_T), t = m - b * a.T;
   const int nn = seq_new(a, b);
   if (t >= nn) return;
-  const int end = seq_len(a, b) - nn + t + 1;
-  // parts: tensor-core items over the prefix, the group over the prefix, the group over the tail
-  const int gi = h - quot(h, a.by_g) * a.g;
-  const int R = m * a.g + gi, Rt = t * a.g + gi;  // among the rows of the key head: all, b's
-  int n0 = 0, pre = 0, tail = 0;
-  if (a.p_splits) {
-    const int chunk = a.one_splits && R >= a.pairs * kPairRows ? a.one_chunk : a.p_chunk;
-    n0 = (min(max(end, 0), a.p_end) + chunk - 1) / chunk;
+  // parts: of the prefix (or of all keys), then of the tail
+  int n1 = 0, tail = 0, first = 0;
+  if (a.tc || a.p_stages) {
+    first = a.shares[row];
+    n1 = a.shares[a.rows + row];
   }
-  if (a.p_stages) pre = a.shares[row];
-  if (!a.by_seq && tail_stages(a, seq_len(a, b)) > 0) tail = a.shares[a.rows + row];
-  const int n1 = n0 + (pre & 0xffff), n2 = n1 + (tail & 0xffff);
+  if (!a.by_seq && tail_stages(a, seq_len(a, b)) > 0) tail = a.shares[2 * a.rows + row];
+  const int n2 = n1 + (tail & 0xffff);
+  const int gi = h - quot(h, a.by_g) * a.g;
+  const int R = (m * a.g + gi) & (kRows - 1), Rt = (t * a.g + gi) & (kRows - 1);  // in their tiles
   auto part = [&](int i) -> int64_t {
-    if (i < n0) return i * a.rows + row;
-    const bool of_tail = i >= n1;
-    const int sh = of_tail ? tail : pre, k = i - (of_tail ? n1 : n0);
-    if ((sh & 0xffff) == 1) return (of_tail ? a.slots - 1 : 0) * a.rows + row;
-    return a.slots * a.rows + (((sh >> 16) + k) * 2 + (k == 0)) * kRows +
-           ((of_tail ? Rt : R) & (kRows - 1));
+    if (i < n1 && a.tc) return first + i * kPairRows;
+    if (i < n1)
+      return n1 == 1 ? a.part_p + row : a.part_f + ((first + i) * 2 + (i == 0)) * kRows + R;
+    i -= n1;
+    return (tail & 0xffff) == 1 ? a.part_t + row
+                                : a.part_f + (((tail >> 16) + i) * 2 + (i == 0)) * kRows + Rt;
   };
   float mx = -INFINITY, l = 0.0f;
   float2 acc = make_float2(0.0f, 0.0f);
@@ -1200,87 +1299,67 @@ __global__ void __launch_bounds__(256)
 namespace {
 
 struct Plan {
-  int tc_items;    // of the tensor-core kernel, 0: not launched
+  int tc_grid;     // CTAs of the tensor-core kernel, 0: not launched
   bool by_seq;     // they cover everything
-  int pairs, p_splits, p_chunk, one_splits, one_chunk, p_end;
-  int grid;        // of the 16-row kernel, 0: not launched
+  int pairs, splits, chunk, per_kv;
+  int grid;        // CTAs of the 16-row kernel, 0: not launched
   int p_tiles, p_stages, whole;
   bool direct;
-  int slots;
-  size_t parts;    // of rows in the workspace
+  int64_t part_p, part_t, part_f, parts;
 };
 
 int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 
-// Keys of a chunk when `groups` items share `keys` keys each: enough items for
-// `want`, chunks of at least min_keys, a multiple of `step`.
-int chunk_keys(int64_t keys, int64_t groups, int64_t want, int min_keys, int step) {
-  const int64_t splits = cdiv(want, groups);
-  const int64_t c = cdiv(cdiv(keys, splits), step) * step;
-  return (int)(c < min_keys ? min_keys : c);
-}
-
-// W8A8_ERR_UNSUPPORTED: more stages than 32 bits count.
+// W8A8_ERR_UNSUPPORTED: more items or stages than 32 bits count.
 int make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared, Plan *out) {
   Plan p = {};
   const int g = n_head / n_kv;
   const int64_t own = (int64_t)T * g, all = own * n_seq;  // rows of a key head
   const int64_t rows = all * n_kv;
-  p.p_end = n_shared;
-  if (own >= 64) {
-    // enough rows a sequence to fill a tile: prefix and tail in one item
+  const int tail = max_ctx - n_shared > 0 ? max_ctx - n_shared : 1;
+  int64_t tc_grid = 0;
+  if (own >= 64 && n_shared < tail) {
+    // rows enough of one sequence to fill a tile, and more keys of its own than shared ones:
+    // prefix and tail in one item. Chunks for two CTAs an SM, of eight blocks at least.
     p.by_seq = true;
     p.pairs = (int)cdiv(own, kPairRows);
     const int64_t groups = (int64_t)n_seq * n_kv * p.pairs;
-    p.p_chunk = chunk_keys(max_ctx, groups, groups >= kSms ? groups : kSms, 4 * kTcKeys, kTcKeys);
-    p.p_splits = (int)cdiv(max_ctx, p.p_chunk);
-    p.p_end = max_ctx;
-    if (groups * p.p_splits > 0x7fffffff) return W8A8_ERR_UNSUPPORTED;
-    p.tc_items = (int)(groups * p.p_splits);
-    p.slots = p.p_splits;
-    p.direct = p.slots == 1;
-    p.parts = p.direct ? 0 : (size_t)rows * p.slots;
-    *out = p;
-    return W8A8_OK;
+    int64_t c = cdiv(cdiv(max_ctx, cdiv(2 * kSms, groups)), kTcKeys) * kTcKeys;
+    p.chunk = (int)(c < 8 * kTcKeys ? 8 * kTcKeys : c);
+    p.splits = (int)cdiv(max_ctx, p.chunk);
+    tc_grid = groups * p.splits;
+    p.direct = p.splits == 1;
+  } else {
+    const int64_t p_stages = cdiv(n_shared, kStageKeys), p_tiles = cdiv(all, kRows);
+    const int64_t t_stages = cdiv(tail, kStageKeys), t_tiles = cdiv(own, kRows);
+    const int64_t pre = n_kv * p_tiles * p_stages;
+    int64_t stages = n_seq * t_tiles * t_stages * n_kv;
+    if (pre > kMinTcStages && all > kRows) {
+      p.per_kv = n_kv < kSms ? kSms / n_kv : 1;
+      const int64_t pairs = cdiv(all, kPairRows);
+      tc_grid = n_kv * (pairs > p.per_kv ? pairs : p.per_kv);
+    } else if (n_shared > 0) {
+      p.p_tiles = (int)p_tiles;
+      p.p_stages = (int)p_stages;
+      stages += pre;
+    } else if (t_stages <= 4) {
+      // short sequences, nothing shared: whole groups, and no join
+      p.whole = (int)t_stages;
+      p.direct = true;
+    }
+    if (stages > 0x7fffffff - kSms * kMmaWarps) return W8A8_ERR_UNSUPPORTED;
+    const int64_t work = p.whole ? stages / p.whole : stages;
+    p.grid = (int)(work < kSms ? work : kSms);
+    p.part_p = tc_grid * kPairRows;
+    p.part_t = p.part_p + (p.p_stages ? rows : 0);
+    p.part_f = p.part_t + rows;
+    // warps with a stretch
+    p.parts = p.part_f + (work < kSms * kMmaWarps ? work : kSms * kMmaWarps) * 2 * kRows;
   }
-  const int64_t p_stages = cdiv(n_shared, kStageKeys), p_tiles = cdiv(all, kRows);
-  const int tail = max_ctx - n_shared > 0 ? max_ctx - n_shared : 1;
-  const int64_t t_stages = cdiv(tail, kStageKeys), t_tiles = cdiv(own, kRows);
-  int64_t stages = n_seq * t_tiles * t_stages * n_kv;
-  const int64_t pre = n_kv * p_tiles * p_stages;
-  if (pre > kMinTcStages && all > kRows) {
-    // full pairs get twice the chunks of a last single tile, whose blocks take half the time;
-    // one CTA an SM in all, if there are that few
-    const int64_t tiles = cdiv(all, kTileRows);
-    p.pairs = (int)(tiles / 2);
-    const int single = (int)(tiles & 1);
-    int64_t per = kSms / n_kv;  // CTAs a key head
-    int64_t s1 = per / (2 * p.pairs + single);
-    if (s1 < 1) s1 = 1;
-    int64_t s2 = p.pairs ? (per - s1 * single) / p.pairs : 0;
-    if (s2 < 1) s2 = 1;
-    p.p_chunk = chunk_keys(n_shared, 1, s2, 2 * kTcKeys, kTcKeys);
-    p.one_chunk = chunk_keys(n_shared, 1, s1, 2 * kTcKeys, kTcKeys);
-    p.p_splits = (int)cdiv(n_shared, p.pairs ? p.p_chunk : p.one_chunk);
-    p.one_splits = single ? (int)cdiv(n_shared, p.one_chunk) : 0;
-    p.tc_items = n_kv * (p.pairs * p.p_splits + p.one_splits);
-    p.slots = p.p_splits > p.one_splits ? p.p_splits : p.one_splits;
-  } else if (n_shared > 0) {
-    p.p_tiles = (int)p_tiles;
-    p.p_stages = (int)p_stages;
-    stages += pre;
-    p.slots = 1;
-  } else if (t_stages <= 4) {
-    // short sequences, nothing shared: whole groups, and no join
-    p.whole = (int)t_stages;
-    p.direct = true;
-  }
-  if (stages > 0x7fffffff - kSms * kMmaWarps) return W8A8_ERR_UNSUPPORTED;
-  const int64_t work = p.whole ? stages / p.whole : stages;
-  p.grid = (int)(work < kSms ? work : kSms);
-  p.slots += 1;
-  const int64_t warps = work < kSms * kMmaWarps ? work : kSms * kMmaWarps;  // with a stretch
-  p.parts = p.direct ? 0 : (size_t)(rows * p.slots + warps * 2 * kRows);
+  if (tc_grid > 0x7fffffff / kPairRows) return W8A8_ERR_UNSUPPORTED;
+  p.tc_grid = (int)tc_grid;
+  if (p.by_seq) p.parts = tc_grid * kPairRows;
+  if (p.direct) p.parts = 0;
   *out = p;
   return W8A8_OK;
 }
@@ -1302,14 +1381,14 @@ int opt_in_smem(K *kernel, size_t bytes, bool (&done)[64]) {
 
 }  // namespace
 
-// Parts of rows (64 sums, a maximum and a sum of weights each), and two words a row.
+// Parts of rows (64 sums, a maximum and a sum of weights each), and three words a row.
 size_t attention_pages_workspace_bytes(int n_seq, int T, int n_head, int n_kv, int max_ctx,
                                        int n_shared) {
   Plan p;
   if (make_plan(n_seq, T, n_head, n_kv, max_ctx, n_shared, &p)) return 0;
   if (p.direct) return 16;
-  return p.parts * (kPageHd * sizeof(float) + sizeof(float2)) +
-         2 * sizeof(int) * (size_t)n_seq * T * n_head;
+  return (size_t)p.parts * (kPageHd * sizeof(float) + sizeof(float2)) +
+         3 * sizeof(int) * (size_t)n_seq * T * n_head;
 }
 
 int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStream_t s) {
@@ -1340,18 +1419,19 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStrea
   a.whole = p.whole;
   a.by_seq = p.by_seq;
   a.pairs = p.pairs;
-  a.p_splits = p.p_splits;
-  a.p_chunk = p.p_chunk;
-  a.one_splits = p.one_splits;
-  a.one_chunk = p.one_chunk;
-  a.p_end = p.p_end;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.per_kv = p.per_kv;
   a.direct = p.direct;
-  a.behind = p.tc_items > 0 && p.grid > 0;
+  a.tc = p.tc_grid > 0;
+  a.behind = a.tc && p.grid > 0;
   a.rows = (int64_t)q.n_seq * q.T * q.n_head;
   a.by_g = make_div(g);
   a.by_T = make_div(q.T);
   a.by_head = make_div(q.n_head);
-  a.slots = p.slots;
+  a.part_p = p.part_p;
+  a.part_t = p.part_t;
+  a.part_f = p.part_f;
   a.Op = reinterpret_cast<float *>(q.ws);
   a.ml = reinterpret_cast<float2 *>(a.Op + p.parts * kPageHd);
   a.shares = reinterpret_cast<int *>(a.ml + p.parts);
@@ -1370,11 +1450,11 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStrea
                                 kPageHd * 2, (uint64_t)c.page_stride * 2, kPageHd, box);
   };
   static bool tc_ready[64], mma_ready[64];
-  if (p.tc_items) {
+  if (p.tc_grid) {
     const size_t smem = 1024 + (2 + 2 * kTcStages) * kTcTile + sizeof(TcCtl);
     st = opt_in_smem(attention_pages_tc_kernel, smem, tc_ready);
     if (st || (st = maps(kBoxRows))) return st;
-    launch_pdl(attention_pages_tc_kernel, dim3((unsigned)p.tc_items), dim3(kTcThreads), smem, s,
+    launch_pdl(attention_pages_tc_kernel, dim3((unsigned)p.tc_grid), dim3(kTcThreads), smem, s,
                tmK, tmV, a);
     st = check_launch("attention_pages_tc");
     if (st) return st;

@@ -90,14 +90,13 @@ def attention(Q, K, V, n_new):
     n, G = K.shape[:2]
     H = Q.shape[1]
     O, A = np.zeros((n_new, H, 64)), np.zeros((n_new, H, 64))
-    for t in range(n_new):
-        end = n - n_new + t + 1
-        if end <= 0:
-            continue
-        for h in range(H):
-            k, v = K[:end, h // (H // G)], V[:end, h // (H // G)]
-            s = k @ Q[t, h] / 8.0
-            w = np.exp(s - s.max())
-            w /= w.sum()
-            O[t, h], A[t, h] = w @ v, w @ np.abs(v)
+    for h in range(H):
+        k, v = K[:, h // (H // G)], V[:, h // (H // G)]
+        s = Q[:n_new, h] @ k.T / 8.0
+        for t in range(n_new):
+            end = n - n_new + t + 1
+            if end > 0:
+                w = np.exp(s[t, :end] - s[t, :end].max())
+                w /= w.sum()
+                O[t, h], A[t, h] = w @ v[:end], w @ np.abs(v[:end])
     return O, A

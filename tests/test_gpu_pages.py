@@ -272,13 +272,24 @@ CASES = [
     (2, 150, 3, 3, 16, 208, [150, 170]),
     (1, 257, 2, 2, 128, 0, [300]),
     (1, 130, 2, 2, 32, 0, [130]),
+    # prefixes long enough, times rows, for the tensor-core kernel: pairs of tiles and a single
+    # one, grouped heads, packed rows of padded batches, empty sequences
+    (300, 1, 8, 8, 64, 1728, [1 + i % 70 for i in range(300)]),
+    (100, 1, 16, 16, 16, 2304, [i % 3 for i in range(100)]),
+    (40, 1, 8, 1, 128, 13056, [3 * i - 1 for i in range(40)]),
+    (5, 40, 12, 4, 32, 1760, [40, 90, -1, 41, 60]),
+    (70, 5, 7, 7, 16, 2000, [5 + i % 9 if i % 7 else -1 for i in range(70)]),
+    (4, 100, 6, 6, 32, 2848, [100, 101, 150, 130]),
+    # more keys of the sequences' own than shared, and rows enough: prefix and tail in one item
+    (2, 70, 4, 2, 32, 64, [70, 2300]),
+    (3, 300, 2, 1, 64, 128, [300, 1500, 400]),
 ]
 
 
 @pytest.mark.parametrize("n_seq,T,H,G,page,n_shared,tails", CASES)
 def test_attention_against_64_bits(cuda, n_seq, T, H, G, page, n_shared, tails):
     n_new = [T if t >= T else max(t, 0) for t in tails]
-    n_new = [min(n, T - b % 3) if T > 3 else n for b, n in enumerate(n_new)]  # a padded batch
+    n_new = [min(n, T - 2 * b % T) if T > 3 else n for b, n in enumerate(n_new)]  # padded
     uniform = T == 1 and all(t >= 1 for t in tails)
     if T == 1 and not uniform:
         n_new = [1 if t >= 0 else 0 for t in tails]
