@@ -57,6 +57,38 @@ __device__ __forceinline__ int quot(int n, const Div &d) {
   return d.mul ? (int)(__umulhi((uint32_t)n, d.mul) >> d.shift) : n;
 }
 
+constexpr int kTileRows = 128, kPairRows = 256;  // tensor-core row tiles
+constexpr int kTcKeys = 128;                     // and keys of a block
+
+// The tensor-core items of a key head over the shared prefix: the rows that hold a query,
+// packed, in pairs of tiles and perhaps a last single one, the keys of a pair in s2 chunks of
+// c2, a single tile's in s1 of c1. A CTA's time goes by its blocks, and a single tile's take
+// half as long, so its chunks are twice as long.
+struct Across {
+  int rows, pairs, s2, c2, s1, c1;  // s1 = 0: no single tile
+  int cost;                         // rounds of CTAs times blocks of one
+};
+// With a pair's keys in about `splits` chunks; of at most max_items in all, if there is a
+// choice. What a CTA does besides its blocks takes the time of three.
+__host__ __device__ inline Across across_of(int rows, int n_kv, int n_shared, int splits,
+                                            int max_items) {
+  Across p = {};
+  const int tiles = (rows + kTileRows - 1) / kTileRows, single = tiles & 1;
+  const int blocks = (n_shared + kTcKeys - 1) / kTcKeys;
+  p.rows = rows;
+  p.pairs = tiles >> 1;
+  const int b2 = (blocks + splits - 1) / splits;
+  const int b1 = p.pairs && 2 * b2 < blocks ? 2 * b2 : p.pairs ? blocks : b2;
+  p.c2 = b2 * kTcKeys;
+  p.c1 = b1 * kTcKeys;
+  p.s2 = p.pairs ? (blocks + b2 - 1) / b2 : 0;
+  p.s1 = single ? (blocks + b1 - 1) / b1 : 0;
+  const int items = n_kv * (p.pairs * p.s2 + p.s1);
+  p.cost = (items + kSms - 1) / kSms * (p.pairs ? b2 + 3 : (b1 + 1) / 2 + 3);
+  if (splits > 1 && items > max_items) p.cost = 0x7fffffff;
+  return p;
+}
+
 struct ApArgs {
   const uint16_t *Q;
   int64_t ldq;
@@ -71,10 +103,11 @@ struct ApArgs {
   int p_tiles, p_stages;
   int whole;           // stages given to every sequence's groups, none split; 0: as many as it has
   // tensor-core items: rows of one sequence over all its keys, [pairs][n_seq][n_kv][splits]
-  // of `chunk` keys; or of all sequences over the prefix, per_kv CTAs a key head (see
-  // plan_across)
-  int by_seq, pairs, splits, chunk, per_kv;
-  int tc;              // the tensor-core kernel runs
+  // of `chunk` keys; or of all sequences over the prefix, as
+  // `across` has them (all T rows of a sequence hold a query), or as plan_across finds
+  int by_seq, pairs, splits, chunk;
+  Across across;
+  int tc;              // CTAs of the tensor-core kernel
   int behind;          // the 16-row kernel runs behind the tensor-core kernel
   int direct;          // every row is one item's or group's, which writes O itself
   int64_t rows;        // n_seq * T * n_head
@@ -90,8 +123,6 @@ struct ApArgs {
   int *shares;
   int *err;
 };
-
-constexpr int kTileRows = 128, kPairRows = 256;  // tensor-core row tiles
 
 __device__ __forceinline__ int seq_len(const ApArgs &a, int b) {
   return min(max(a.n_ctx[b], 0), a.max_ctx);
@@ -668,7 +699,6 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
 // ---------------------------------------------------------------------------
 namespace {
 
-constexpr int kTcKeys = 128;
 constexpr int kBoxRows = 64;  // at most, of a TMA box
 constexpr int kTcStages = 5;
 constexpr uint32_t kTcTile = kTcKeys * 128;  // Q tile, or K or V of a block: 16 KB
@@ -697,42 +727,21 @@ struct TcItem {
   int split, splits;  // of the rows' items over their keys
 };
 
-// The prefix items of a key head: the rows that hold a query, packed (their number is known
-// here only), in pairs of tiles and perhaps a last single one. A CTA's time goes by its
-// blocks, and a single tile's take half as long, so its items get twice the keys; one CTA an
-// SM in all if the rows are few.
-struct Across {
-  int rows, pairs, s2, c2, s1, c1;  // s1 = 0: no single tile
-};
 __device__ __forceinline__ Across plan_across(const ApArgs &a, int lane) {
-  Across p;
-  int valid = a.n_seq * a.T;
-  if (a.n_new) {
-    valid = 0;
+  if (!a.n_new) return a.across;
+  int valid = 0;
 #pragma unroll 4
-    for (int b = lane; b < a.n_seq; b += 32) valid += seq_new(a, b);
+  for (int b = lane; b < a.n_seq; b += 32) valid += seq_new(a, b);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) valid += __shfl_xor_sync(~0u, valid, d);
-  }
-  p.rows = valid * a.g;
-  const int tiles = (p.rows + kTileRows - 1) / kTileRows, single = tiles & 1;
-  p.pairs = tiles >> 1;
-  auto chunk = [&](int splits) {
-    const int c = ((a.n_shared + splits - 1) / splits + kTcKeys - 1) / kTcKeys * kTcKeys;
-    return max(c, 2 * kTcKeys);
-  };
-  p.s1 = p.s2 = 0;
-  p.c1 = p.c2 = kTcKeys;
-  if (tiles == 0) return p;
-  const int s1 = max(1, a.per_kv / tiles);
-  if (single) {
-    p.c1 = chunk(s1);
-    p.s1 = (a.n_shared + p.c1 - 1) / p.c1;
-  }
-  if (p.pairs) {
-    p.c2 = chunk(max(1, (a.per_kv - s1 * single) / p.pairs));
-    p.s2 = (a.n_shared + p.c2 - 1) / p.c2;
-  }
+  for (int d = 16; d; d >>= 1) valid += __shfl_xor_sync(~0u, valid, d);
+  Across p = across_of(valid * a.g, a.n_kv, a.n_shared, lane + 1, a.tc);
+  int best = min(p.cost, 1 << 25) << 5 | lane;  // a lane a choice
+#pragma unroll
+  for (int d = 16; d; d >>= 1) best = min(best, __shfl_xor_sync(~0u, best, d));
+  p.c2 = __shfl_sync(~0u, p.c2, best & 31);
+  p.s2 = __shfl_sync(~0u, p.s2, best & 31);
+  p.c1 = __shfl_sync(~0u, p.c1, best & 31);
+  p.s1 = __shfl_sync(~0u, p.s1, best & 31);
   return p;
 }
 
@@ -1219,30 +1228,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// The join of a row's parts, a warp a row: a lane a part for the weights, then
-// two dims a lane, eight parts' loads in flight.
+// The join of a row's parts: eight lanes, eight dims a lane, four parts' loads in
+// flight; SUB = 4 such groups share a row's parts where there are few rows, since
+// a row's chain of dependent reads (length, words of the row, parts) is the time
+// of the kernel then.
 // ---------------------------------------------------------------------------
+template <int SUB>
 __global__ void __launch_bounds__(256)
     attention_pages_join_kernel(const __grid_constant__ ApArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr int kLanes = 8 * SUB;
+  const int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int d0 = (threadIdx.x & 7) * 8, sub = threadIdx.x / 8 % SUB;
   pdl_launch_dependents();
   pdl_wait();
   if (row >= a.rows) return;
-  const int m = quot(row, a.by_head), h = row - m * (a.n_kv * a.g);
+  const int m = quot((int)row, a.by_head), h = (int)row - m * (a.n_kv * a.g);
   const int b = quot(m, a.by_T), t = m - b * a.T;
-  const int nn = seq_new(a, b);
-  if (t >= nn) return;
-  // parts: of the prefix (or of all keys), then of the tail
-  int n1 = 0, tail = 0, first = 0;
-  if (a.tc || a.p_stages) {
-    first = a.shares[row];
-    n1 = a.shares[a.rows + row];
-  }
-  if (!a.by_seq && tail_stages(a, seq_len(a, b)) > 0) tail = a.shares[2 * a.rows + row];
+  // words of a row are read before it is known which of them hold anything
+  const int first = a.shares[row], n_first = a.shares[a.rows + row];
+  const int tail_word = a.shares[2 * a.rows + row];
+  if (t >= seq_new(a, b)) return;
+  const int n1 = a.tc || a.p_stages ? n_first : 0;
+  const int tail = !a.by_seq && tail_stages(a, seq_len(a, b)) > 0 ? tail_word : 0;
   const int n2 = n1 + (tail & 0xffff);
   const int gi = h - quot(h, a.by_g) * a.g;
   const int R = (m * a.g + gi) & (kRows - 1), Rt = (t * a.g + gi) & (kRows - 1);  // in their tiles
+  // parts: of the prefix (or of all keys), then of the tail
   auto part = [&](int i) -> int64_t {
     if (i < n1 && a.tc) return first + i * kPairRows;
     if (i < n1)
@@ -1251,46 +1262,57 @@ __global__ void __launch_bounds__(256)
     return (tail & 0xffff) == 1 ? a.part_t + row
                                 : a.part_f + (((tail >> 16) + i) * 2 + (i == 0)) * kRows + Rt;
   };
-  float mx = -INFINITY, l = 0.0f;
-  float2 acc = make_float2(0.0f, 0.0f);
-  for (int base = 0; base < n2; base += 32) {
-    const bool live = base + lane < n2;
-    const int64_t at = live ? part(base + lane) : 0;
-    const float2 v = live ? a.ml[at] : make_float2(-INFINITY, 0.0f);
-    float top = v.x;
+  float mx = -INFINITY, l = 0.0f, acc[8] = {};
+  for (int i0 = 4 * sub; i0 < n2; i0 += 4 * SUB) {
+    float2 v[4];
+    float4 x[4][2];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    top = fmaxf(top, mx);
-    const float ms = safe_max(top), f = ex2(mx - ms), w = live ? ex2(v.x - ms) : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+      const bool live = i0 + i < n2;
+      const int64_t at = live ? part(i0 + i) : 0;
+      const float4 *src = reinterpret_cast<const float4 *>(a.Op + at * kPageHd + d0);
+      v[i] = live ? a.ml[at] : make_float2(-INFINITY, 0.0f);
+      x[i][0] = live ? src[0] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      x[i][1] = live ? src[1] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    const float top = fmaxf(fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)), mx);
+    const float ms = safe_max(top), f = ex2(mx - ms);
     mx = top;
-    l = l * f + w * v.y;  // this lane's parts
-    acc.x *= f;
-    acc.y *= f;
-    const int n = min(32, n2 - base);
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float2 x[8];
-      float wx[8];
+    l *= f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = k0 + i;
-        wx[i] = __shfl_sync(~0u, w, k & 31);
-        const int64_t from = __shfl_sync(~0u, at, k & 31);
-        x[i] = k < n ? reinterpret_cast<const float2 *>(a.Op + from * kPageHd)[lane]
-                     : make_float2(0.0f, 0.0f);
-      }
+    for (int d = 0; d < 8; ++d) acc[d] *= f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k0 + i < n) {
-          acc.x += wx[i] * x[i].x;
-          acc.y += wx[i] * x[i].y;
-        }
+    for (int i = 0; i < 4; ++i) {
+      if (i0 + i >= n2) break;
+      const float w = ex2(v[i].x - ms);
+      l += w * v[i].y;
+      const float y[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w,
+                          x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
+#pragma unroll
+      for (int d = 0; d < 8; ++d) acc[d] += w * y[d];
     }
   }
+  if constexpr (SUB > 1) {  // (a row is left by all of a warp or by none)
+    static_assert(kLanes == 32, "a warp a row");
 #pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+    for (int x = 8; x < kLanes; x *= 2) {
+      const float other = __shfl_xor_sync(~0u, mx, x), top = fmaxf(mx, other);
+      const float f = ex2(mx - safe_max(top));
+      mx = top;
+      l *= f;
+      l += __shfl_xor_sync(~0u, l, x);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        acc[d] *= f;
+        acc[d] += __shfl_xor_sync(~0u, acc[d], x);
+      }
+    }
+    if (sub != 0) return;
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  reinterpret_cast<uint32_t *>(a.O + (int64_t)m * a.ldo + h * kPageHd)[lane] =
-      pack_bf2(acc.x * inv, acc.y * inv);
+  uint32_t *dst = reinterpret_cast<uint32_t *>(a.O + m * a.ldo + h * kPageHd + d0);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) dst[d] = pack_bf2(acc[2 * d] * inv, acc[2 * d + 1] * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -1301,7 +1323,7 @@ namespace {
 struct Plan {
   int tc_grid;     // CTAs of the tensor-core kernel, 0: not launched
   bool by_seq;     // they cover everything
-  int pairs, splits, chunk, per_kv;
+  int pairs, splits, chunk;
   int grid;        // CTAs of the 16-row kernel, 0: not launched
   int p_tiles, p_stages, whole;
   bool direct;
@@ -1335,9 +1357,9 @@ int make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared,
     const int64_t pre = n_kv * p_tiles * p_stages;
     int64_t stages = n_seq * t_tiles * t_stages * n_kv;
     if (pre > kMinTcStages && all > kRows) {
-      p.per_kv = n_kv < kSms ? kSms / n_kv : 1;
-      const int64_t pairs = cdiv(all, kPairRows);
-      tc_grid = n_kv * (pairs > p.per_kv ? pairs : p.per_kv);
+      // a CTA for each pair at least, and room for two rounds of them
+      tc_grid = n_kv * cdiv(all, kPairRows);
+      if (tc_grid < 2 * kSms) tc_grid = 2 * kSms;
     } else if (n_shared > 0) {
       p.p_tiles = (int)p_tiles;
       p.p_stages = (int)p_stages;
@@ -1421,10 +1443,18 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStrea
   a.pairs = p.pairs;
   a.splits = p.splits;
   a.chunk = p.chunk;
-  a.per_kv = p.per_kv;
   a.direct = p.direct;
-  a.tc = p.tc_grid > 0;
-  a.behind = a.tc && p.grid > 0;
+  a.tc = p.tc_grid;
+  if (p.tc_grid && !p.by_seq && !q.n_new) {
+    // every row holds a query: the items, and no CTA more, are known here
+    a.across = across_of(q.n_seq * q.T * g, a.n_kv, a.n_shared, 1, a.tc);
+    for (int i = 2; i <= 32; ++i) {
+      const Across x = across_of(q.n_seq * q.T * g, a.n_kv, a.n_shared, i, a.tc);
+      if (x.cost < a.across.cost) a.across = x;
+    }
+    p.tc_grid = a.n_kv * (a.across.pairs * a.across.s2 + a.across.s1);
+  }
+  a.behind = p.tc_grid > 0 && p.grid > 0;
   a.rows = (int64_t)q.n_seq * q.T * q.n_head;
   a.by_g = make_div(g);
   a.by_T = make_div(q.T);
@@ -1468,7 +1498,12 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStrea
     if (st) return st;
   }
   if (a.direct) return W8A8_OK;
-  launch_pdl(attention_pages_join_kernel, dim3((unsigned)cdiv(a.rows, 8)), dim3(256), 0, s, a);
+  // four groups a row as long as they all run at once (eight CTAs an SM)
+  if (a.rows <= (int64_t)kSms * 8 * 8)
+    launch_pdl(attention_pages_join_kernel<4>, dim3((unsigned)cdiv(a.rows, 8)), dim3(256), 0, s, a);
+  else
+    launch_pdl(attention_pages_join_kernel<1>, dim3((unsigned)cdiv(a.rows, 32)), dim3(256), 0, s,
+               a);
   return check_launch("attention_pages_join");
 }
 
