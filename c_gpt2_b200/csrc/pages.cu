@@ -158,49 +158,57 @@ __global__ void __launch_bounds__(kBookThreads)
 }
 
 // ---------------------------------------------------------------------------
-// write: row t of sequence b at position pos0[b] + t of its pages, a 16-byte
-// unit a thread: every row's head segments are 128 contiguous bytes on both
-// sides. Bound by the bytes (latency for a decode step).
+// write: row t of sequence b at position pos0[b] + t of its pages. A warp takes a
+// row's keys or its values, so that the place is worked out once a row (with four
+// divisions a 16-byte unit instead, the kernel was bound by issue: 27 us for 16
+// prompts of up to 1000 rows of 20 heads, whose bytes take 12.5); a head's segment
+// is 128 contiguous bytes on both sides, and four units a lane are in flight.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
     pages_write_kernel(PagesArgs a, int64_t layer_off, const uint16_t *Kn, int64_t ldk,
                        const uint16_t *Vn, int64_t ldv, int n_seq, int T, const int32_t *n_new,
                        const int32_t *pos0) {
-  const int unit_row = a.n_kv_head * 8;  // 16-byte units of a row
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t m = u / (2 * unit_row);
+  const int64_t x = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int64_t m = x >> 1;
+  const bool is_v = x & 1;
   pdl_launch_dependents();
   pdl_wait();
   if (m >= (int64_t)n_seq * T) return;
-  const int b = (int)(m / T), t = (int)(m - (int64_t)b * T);
-  int w = (int)(u - m * (2 * unit_row));
-  const bool is_v = w >= unit_row;
-  if (is_v) w -= unit_row;
+  const int b = (int)((uint32_t)m / (uint32_t)T), t = (int)m - b * T;
   const int p0 = pos0[b];
   if (p0 < 0 || (n_new && t >= n_new[b])) return;
-  const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(is_v ? Vn + m * ldv : Kn + m * ldk) + w);
   const int64_t pos = (int64_t)p0 + t;
-  const int64_t k = pos / a.page;
-  if (k >= a.max_pages) {
-    report_error(a.err, kErrPos);
+  const int shift = __ffs(a.page) - 1;
+  if (pos >> shift >= a.max_pages) {
+    if (lane == 0) report_error(a.err, kErrPos);
     return;
   }
-  const int p = a.table[(int64_t)b * a.max_pages + k];
+  const int p = a.table[(int64_t)b * a.max_pages + (pos >> shift)];
   if (p < 0 || p >= a.n_pages) {
-    report_error(a.err, kErrPage);
+    if (lane == 0) report_error(a.err, kErrPage);
     return;
   }
-  const int h = w >> 3;
-  uint16_t *pool = is_v ? a.V : a.K;
-  const int64_t off = (int64_t)p * a.page_stride + layer_off +
-                      ((int64_t)h * a.page + (pos - k * a.page)) * kPageHd;
-  reinterpret_cast<uint4 *>(pool + off)[w & 7] = v;
+  const uint4 *from = reinterpret_cast<const uint4 *>(is_v ? Vn + m * ldv : Kn + m * ldk);
+  uint4 *to = reinterpret_cast<uint4 *>((is_v ? a.V : a.K) + (int64_t)p * a.page_stride +
+                                        layer_off + (pos & (a.page - 1)) * kPageHd);
+  const int n = a.n_kv_head * 8;
+  for (int w0 = lane; w0 < n; w0 += 128) {
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (w0 + 32 * j < n) v[j] = __ldcs(from + w0 + 32 * j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int w = w0 + 32 * j;
+      if (w < n) to[(int64_t)(w >> 3) * (a.page * 8) + (w & 7)] = v[j];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
 // fork, first kernel: which entries of the list hold, and a page for each
-// whose source ends inside one. Second kernel: the shared pages' entries and
-// counts, and the rows that the last page holds.
+// whose source ends inside one.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(kBookThreads)
     pages_fork_book_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n,
@@ -251,52 +259,60 @@ __global__ void __launch_bounds__(kBookThreads)
   }
 }
 
+// The whole pages' entries and counts, an entry of the list a CTA; then the rows
+// that the last pages hold: a CTA takes a piece of a page (four 16-byte
+// units a thread, of both pools in turn) and copies it for its share of the list,
+// keeping what it read while the source stays the same: for the forks of one
+// sequence nothing but the writes is left.
 __global__ void __launch_bounds__(256)
-    pages_fork_copy_kernel(PagesArgs a, const int32_t *src, const int32_t *dst,
+    pages_fork_rows_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n,
                            const int32_t *status) {
-  const int i = blockIdx.y;
-  const int tid = blockIdx.x * 256 + threadIdx.x, n_thread = gridDim.x * 256;
   pdl_launch_dependents();
   pdl_wait();
-  if (status[i] != W8A8_FORK_OK) return;
-  const int n = a.n_ctx[dst[i]];
-  const int32_t *from = a.table + (int64_t)src[i] * a.max_pages;
-  int32_t *to = a.table + (int64_t)dst[i] * a.max_pages;
-  const int whole = n / a.page, rows = n % a.page;
-  for (int k = tid; k < whole; k += n_thread) {
-    const int p = from[k];
-    to[k] = p;
-    if (p >= 0 && p < a.n_pages) atomicAdd(&a.refs[p], 1);
-    else report_error(a.err, kErrPage);
+  for (int i = blockIdx.y * gridDim.x + blockIdx.x; i < n; i += gridDim.x * gridDim.y) {
+    if (status[i] != W8A8_FORK_OK) continue;
+    const int whole = a.n_ctx[dst[i]] / a.page;
+    for (int k = threadIdx.x; k < whole; k += 256) {
+      const int p = a.table[(int64_t)src[i] * a.max_pages + k];
+      a.table[(int64_t)dst[i] * a.max_pages + k] = p;
+      if (p >= 0 && p < a.n_pages) atomicAdd(&a.refs[p], 1);
+      else report_error(a.err, kErrPage);
+    }
   }
-  if (rows == 0) return;
-  const int pf = from[whole], pt = to[whole];
-  if (pf < 0 || pf >= a.n_pages || pt < 0 || pt >= a.n_pages) {
-    if (tid == 0) report_error(a.err, kErrPage);
-    return;
-  }
-  // rows * 8 units of 16 bytes in each (layer, head) segment
-  const int seg_units = rows * 8, n_unit = a.n_layer * a.n_kv_head * seg_units;
-  const int64_t seg_stride = (int64_t)a.page * 8;
-#pragma unroll 1
-  for (int pool = 0; pool < 2; ++pool) {
-    uint16_t *base = pool ? a.V : a.K;
-    const uint4 *f = reinterpret_cast<const uint4 *>(base + (int64_t)pf * a.page_stride);
-    uint4 *d = reinterpret_cast<uint4 *>(base + (int64_t)pt * a.page_stride);
-    for (int u = tid; u < n_unit; u += 4 * n_thread) {
-      uint4 v[4];
-      int64_t at[4];
+  const bool is_v = blockIdx.x & 1;
+  uint4 *pool = reinterpret_cast<uint4 *>(is_v ? a.V : a.K);
+  const int64_t stride = a.page_stride / 8;
+  const int u0 = (blockIdx.x >> 1) * 1024 + threadIdx.x;
+  int held = -1, held_rows = 0;  // page and rows in v
+  uint4 v[4];
+  int64_t at[4];
+  bool live[4];
+  for (int i = blockIdx.y; i < n; i += gridDim.y) {
+    if (status[i] != W8A8_FORK_OK) continue;
+    const int len = a.n_ctx[dst[i]], whole = len / a.page, rows = len % a.page;
+    if (rows == 0) continue;
+    const int pf = a.table[(int64_t)src[i] * a.max_pages + whole];
+    const int pt = a.table[(int64_t)dst[i] * a.max_pages + whole];
+    if (pf < 0 || pf >= a.n_pages || pt < 0 || pt >= a.n_pages) {
+      if (threadIdx.x == 0) report_error(a.err, kErrPage);
+      continue;
+    }
+    if (pf != held || rows != held_rows) {
+      // rows * 8 units in each (layer, head) segment of the page
+      const int seg_units = rows * 8, n_unit = a.n_layer * a.n_kv_head * seg_units;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int x = u + j * n_thread;
-        const int seg = x / seg_units;
-        at[j] = seg * seg_stride + (x - seg * seg_units);
-        if (x < n_unit) v[j] = f[at[j]];
+        const int x = u0 + j * 256, seg = x / seg_units;
+        live[j] = x < n_unit;
+        at[j] = (int64_t)seg * a.page * 8 + (x - seg * seg_units);
+        if (live[j]) v[j] = pool[pf * stride + at[j]];
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (u + j * n_thread < n_unit) d[at[j]] = v[j];
+      held = pf;
+      held_rows = rows;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (live[j]) __stcs(pool + pt * stride + at[j], v[j]);
   }
 }
 
@@ -482,9 +498,9 @@ int launch_pages_extend(const PagesArgs &a, const int32_t *n_new, int32_t *pos0,
 int launch_pages_write(const PagesArgs &a, int layer, const uint16_t *Kn, int64_t ldk,
                        const uint16_t *Vn, int64_t ldv, int n_seq, int T, const int32_t *n_new,
                        const int32_t *pos0, cudaStream_t s) {
-  const int64_t units = (int64_t)n_seq * T * a.n_kv_head * 16;
-  const int64_t blocks = (units + 255) / 256;
-  if (blocks > 0x7fffffff) return W8A8_ERR_UNSUPPORTED;
+  const int64_t warps = 2 * (int64_t)n_seq * T;
+  if (warps > 0x7fffffff) return W8A8_ERR_UNSUPPORTED;
+  const int64_t blocks = (warps + 7) / 8;
   launch_pdl(pages_write_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a,
              (int64_t)layer * a.n_kv_head * a.page * kPageHd, Kn, ldk, Vn, ldv, n_seq, T, n_new,
              pos0);
@@ -499,13 +515,14 @@ int launch_pages_fork(const PagesArgs &a, const int32_t *src, const int32_t *dst
   launch_pdl(pages_fork_book_kernel, dim3(1), dim3(kBookThreads), smem, s, a, src, dst, n, status);
   st = check_launch("pages_fork_book");
   if (st) return st;
-  // eight CTAs an SM over all entries, no more than a fully copied page has work for
+  // a CTA for every piece of a page, and shares of the list for eight an SM
   const int64_t units = (int64_t)a.n_layer * a.n_kv_head * a.page * 8;
-  int64_t x = ((int64_t)sm_count * 8 + n - 1) / n;
-  if (x > (units + 1023) / 1024) x = (units + 1023) / 1024;
-  launch_pdl(pages_fork_copy_kernel, dim3((unsigned)x, (unsigned)n), dim3(256), 0, s, a, src, dst,
-             status);
-  return check_launch("pages_fork_copy");
+  const int64_t x = 2 * ((units + 1023) / 1024);
+  int64_t y = ((int64_t)sm_count * 8 + x - 1) / x;
+  if (y > n) y = n;
+  launch_pdl(pages_fork_rows_kernel, dim3((unsigned)x, (unsigned)y), dim3(256), 0, s, a, src, dst,
+             n, status);
+  return check_launch("pages_fork_rows");
 }
 
 int launch_pages_free(const PagesArgs &a, const int32_t *slots, int n, cudaStream_t s) {

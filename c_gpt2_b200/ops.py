@@ -8,6 +8,7 @@ function has a counterpart there.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -479,6 +480,11 @@ def pages_copy(Ksrc, Vsrc, src, Kdst, Vdst, dst):
         "w8a8_pages_copy")
 
 
+@functools.lru_cache(maxsize=4096)
+def _attention_pages_workspace(*sizes: int) -> int:
+    return core().w8a8_attention_pages_workspace_size(*sizes)
+
+
 def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shared_pages=None,
                     n_shared=0, out=None, workspace=None):
     """Attention of the T newest positions of each sequence over its pages: rows
@@ -497,9 +503,8 @@ def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shar
     O = out if out is not None else Q.new_empty((n_seq * T, d))
     o, ldo = _rows(O, n_seq * T, d, dev, "out")
     if workspace is None:
-        need = core().w8a8_attention_pages_workspace_size(n_seq, T, n_head, cache.n_kv_head,
-                                                          max_ctx, n_shared)
-        workspace = torch.empty(need, dtype=_U8, device=cache.device)
+        workspace = torch.empty(_attention_pages_workspace(n_seq, T, n_head, cache.n_kv_head,
+                                                           max_ctx, n_shared), dtype=_U8, device=cache.device)
     check(core().w8a8_attention_pages(
         cache.ref, layer, q, ldq, n_seq, T,
         None if n_new is None else _here(n_new, _I32, dev, "n_new", n_seq), max_ctx,
