@@ -32,7 +32,7 @@ constexpr int kErrWaitFull = 0x1602;
 constexpr int kStageKeys = 64;
 constexpr int kStages = 2;                         // of each warp
 constexpr uint32_t kTileBytes = kStageKeys * 128;  // keys or values of a stage
-constexpr int kMmaWarps = 6;                       // one CTA an SM, a warp an item
+constexpr int kMmaWarps = 7;                       // one CTA an SM, a warp an item
 constexpr int kRows = 16;                          // query rows of an item
 // A prefix of more 16-row stages than this goes to the tensor-core kernel, if it takes several
 // row tiles. That kernel has a fixed cost of some 8 us; the 16-row kernel, whose re-reads hit
@@ -687,9 +687,11 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
 //   0-3, 4-7  softmax of group 0 and 1: a thread a row (TMEM lane), the row's
 //             128 scores of a block in registers
 //   8         TMA (a box a page, or 64 rows of a larger one)
-//   9         owns TMEM, issues the MMAs: S = Q K^T (128 columns), then
+//   9, 10     issue the MMAs of group 0 and 1: S = Q K^T (128 columns), then
 //             O += P V with P read from TMEM, where the softmax left it as bf16,
 //             so that neither P nor its re-reads pass through shared memory
+//             (one thread for both groups was late for each: S and O came 400
+//             cycles after they were wanted, of 3400 a block); 9 owns TMEM
 // Each group has S (128 columns), P (64) and O (64): all 512 columns. S is free
 // once a group holds it in registers, so S of the next block is formed while
 // the exponentials of this one run, and the groups' MMAs overlap each other's
@@ -704,7 +706,7 @@ constexpr int kBoxRows = 64;  // at most, of a TMA box
 constexpr int kTcStages = 5;
 constexpr uint32_t kTcTile = kTcKeys * 128;  // Q tile, or K or V of a block: 16 KB
 constexpr int kTcTmaWarp = 8, kTcMmaWarp = 9;
-constexpr int kTcThreads = 12 * 32;  // three warpgroups; the last two warps only pass registers
+constexpr int kTcThreads = 12 * 32;  // three warpgroups; the last warp only passes registers
 constexpr int kTcSoftThreads = 8 * 32;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 192, kColGroup = 256;
 constexpr int kErrTc = 0x1610;
@@ -864,7 +866,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&ctl->q_full, 8);
     for (int i = 0; i < kTcStages; ++i) {
       mbar_init(&ctl->kv_full[i], 1);
-      mbar_init(&ctl->kv_empty[i], 1);
+      mbar_init(&ctl->kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->s_full[i], 1);
@@ -874,7 +876,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int i = 0; i < 8; ++i) mbar_init(&ctl->turn[i >> 2][i & 3], 1);
     mbar_init(&ctl->v_ready, 1);
-    mbar_init(&ctl->drain, 1);
+    mbar_init(&ctl->drain, 2);
     ctl->abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmK);
@@ -956,12 +958,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       float mx[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = max3(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]), -INFINITY);
+      for (int c = 0; c < 4; ++c)
+        mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-        for (int k = 2; k < 32; k += 2)
+      for (int k = 2; k < 32; k += 2)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
           mx[c] = max3(mx[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-      }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool up = grown(top, m);
       float f = 1.0f;
@@ -996,7 +999,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // (a warp issues in order and would otherwise wait for each). Scaling and sums work on
       // pairs (f32x2).
       const F2 scale2 = f2(kScale2, kScale2), minus = f2(-ms, -ms);
-      F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+      F2 sum[4] = {0, 0, 0, 0};  // (of zeros)
+      uint32_t p[2][32];
       auto pair = [&](int c, int k) {
         return f2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       };
@@ -1008,17 +1012,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       auto scale = [&](int c, int k) { put(c, k, f2_fma(pair(c, k), scale2, minus)); };
       auto take = [&](int c, int k) {  // keys k, k + 1
-        sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], pair(c, k));
-        s[c][k / 2] = pack_bf2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-      };
-      auto store = [&](int c) {  // chunks c - 1 and c
-        uint32_t p[32];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          p[k] = s[c - 1][k];
-          p[16 + k] = s[c][k];
-        }
-        tmem_st_32x32b_x32(trow + kColP + 16 * (c - 1), p);
+        sum[(k >> 1) & 3] = f2_add(sum[(k >> 1) & 3], pair(c, k));
+        p[c >> 1][16 * (c & 1) + k / 2] =
+            pack_bf2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       };
 #pragma unroll
       for (int k = 0; k < 32; k += 2) scale(0, k);
@@ -1031,15 +1027,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (c < 3) scale(c + 1, k);
           if (c > 0) take(c - 1, k);
         }
-        if (c == 2) store(1);
+        if (c == 2) tmem_st_32x32b_x32(trow + kColP, p[0]);
       }
       if (turns && lane == 0) mbar_arrive(&ctl->turn[g ^ 1][qd]);
 #pragma unroll
       for (int k = 0; k < 32; k += 2) take(3, k);
-      store(3);
+      tmem_st_32x32b_x32(trow + kColP + 32, p[1]);
       {
         float x, y;
-        f2_split(f2_add(sum[0], sum[1]), x, y);
+        f2_split(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), x, y);
         l += x + y;
       }
       tmem_st_wait();
@@ -1168,50 +1164,53 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (*abort_flag)  // no copy may still be writing shared memory when the CTA exits
       for (int i = n > kTcStages ? n - kTcStages : 0; i < n; ++i)
         mbar_wait(&ctl->kv_full[i % kTcStages], (i / kTcStages) & 1, nullptr, a.err, kErrTc + 1);
-  } else if (warp == kTcMmaWarp) {
-    // ---------------- MMA: one thread ----------------
+  } else if (warp == kTcMmaWarp || warp == kTcMmaWarp + 1) {
+    // ---------------- MMA of one group: one thread ----------------
+    const int g = warp - kTcMmaWarp;
     if (elect_one()) {
       const uint32_t idS = make_idesc(1, 1, kTileRows, kTcKeys);
       const uint32_t idO = make_idesc_bmn(1, 1, kTileRows, kPageHd);
-      const uint64_t q_desc = make_sw128_desc(smem_u32(sQ));
+      const uint64_t q_desc = make_sw128_desc(smem_u32(sQ)) + (one ? 0 : g) * (kTcTile >> 4);
       const uint64_t k_desc = make_sw128_desc(smem_u32(sKV));
       const uint64_t v_desc = make_sw128_mn_desc(smem_u32(sKV) + kTcTile);
-      bool ok = mbar_wait(&ctl->q_full, 0, abort_flag, a.err, kErrTc + 2);
-      int seen = 0;  // blocks known to be in shared memory
-      auto issue_s = [&](int u) -> bool {
-        const int g = u & 1, i = u >> 1, j = one ? u : i;  // group, its unit, block
+      const uint32_t base = tmem + g * kColGroup;
+      const int mine = (units - g + 1) / 2;
+      bool ok = mine > 0 && mbar_wait(&ctl->q_full, 0, abort_flag, a.err, kErrTc + 2);
+      int seen = 0;  // blocks that have been in shared memory
+      auto issue_s = [&](int i) -> bool {
+        const int j = one ? 2 * i + g : i;  // block
         if (i > 0 && !mbar_wait(&ctl->s_free[g], (i - 1) & 1, abort_flag, a.err, kErrTc + 3))
           return false;
-        const int st = j % kTcStages;
-        if (j >= seen) {
-          if (!mbar_wait(&ctl->kv_full[st], (j / kTcStages) & 1, abort_flag, a.err, kErrTc + 4))
+        for (;; ++seen) {
+          const int st = seen % kTcStages;
+          if (!mbar_wait(&ctl->kv_full[st], (seen / kTcStages) & 1, abort_flag, a.err, kErrTc + 4))
             return false;
-          seen = j + 1;
+          if (seen == j) break;
+          mbar_arrive(&ctl->kv_empty[st]);  // the other group's: a stage is freed by both
         }
+        ++seen;
         tc_fence_after();
-        tc_mma_bf16_x4(tmem + g * kColGroup + kColS, q_desc + (one ? 0 : g) * (kTcTile >> 4),
-                       k_desc + st * (2 * kTcTile >> 4), idS);
+        tc_mma_bf16_x4(base + kColS, q_desc, k_desc + (j % kTcStages) * (2 * kTcTile >> 4), idS);
         tc_commit(&ctl->s_full[g]);
         return true;
       };
-      auto issue_o = [&](int u) -> bool {
-        const int g = u & 1, i = u >> 1, j = one ? u : i;
+      auto issue_o = [&](int i) -> bool {
+        const int j = one ? 2 * i + g : i;
         if (!mbar_wait(&ctl->p_full[g], i & 1, abort_flag, a.err, kErrTc + 5)) return false;
         if (v_cut && j == blocks - 1 &&
             !mbar_wait(&ctl->v_ready, 0, abort_flag, a.err, kErrTc + 10))
           return false;
         tc_fence_after();
-        const uint32_t base = tmem + g * kColGroup;
         tc_mma_bf16_ta_x8(base + kColO, base + kColP, v_desc + (j % kTcStages) * (2 * kTcTile >> 4),
                           idO, i > 0);
         tc_commit(&ctl->o_done[g]);
-        if (one || g == 1) tc_commit(&ctl->kv_empty[j % kTcStages]);
+        tc_commit(&ctl->kv_empty[j % kTcStages]);
         return true;
       };
-      for (int u = 0; u < 2 && u < units && ok; ++u) ok = issue_s(u);
-      for (int u = 0; u < units && ok; u += 2) {
-        for (int v = u + 2; v < u + 4 && v < units && ok; ++v) ok = issue_s(v);
-        for (int v = u; v < u + 2 && v < units && ok; ++v) ok = issue_o(v);
+      if (ok) ok = issue_s(0);
+      for (int i = 0; i < mine && ok; ++i) {
+        if (i + 1 < mine) ok = issue_s(i + 1);
+        if (ok) ok = issue_o(i);
       }
       // no MMA may still be writing TMEM when it is released
       tc_commit(&ctl->drain);
