@@ -1340,9 +1340,15 @@ int make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared,
   const int64_t rows = all * n_kv;
   const int tail = max_ctx - n_shared > 0 ? max_ctx - n_shared : 1;
   int64_t tc_grid = 0;
-  if (own >= 64 && n_shared < tail) {
-    // rows enough of one sequence to fill a tile, and more keys of its own than shared ones:
-    // prefix and tail in one item. Chunks for two CTAs an SM, of eight blocks at least.
+  // A sequence's rows over prefix and tail in one tensor-core item, or all rows over the prefix
+  // and the tails to the 16-row kernel: by the time that one SM takes, where a 128 x 128 block
+  // counts as 5.5 stages of 16 rows by 64 keys (1640 cycles, and some 300 with seven warps).
+  const int64_t heads = (int64_t)n_seq * n_kv;
+  const int64_t one_item = heads * cdiv(own, kTileRows) * cdiv(n_shared + tail, kTcKeys) * 11;
+  const int64_t two_items = n_kv * cdiv(all, kTileRows) * cdiv(n_shared, kTcKeys) * 11 +
+                            heads * cdiv(own, kRows) * cdiv(tail, kStageKeys) * 2;
+  if (own > 2 * kRows && one_item < two_items) {
+    // Chunks for two CTAs an SM, of eight blocks at least.
     p.by_seq = true;
     p.pairs = (int)cdiv(own, kPairRows);
     const int64_t groups = (int64_t)n_seq * n_kv * p.pairs;

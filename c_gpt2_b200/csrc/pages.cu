@@ -102,6 +102,11 @@ __device__ __forceinline__ int owner_of(const int *upto, int n, int rank) {
 
 __device__ __forceinline__ int pages_of(int n, int page) { return (n + page - 1) / page; }
 
+// Positions that a slot may hold: those of its table row, and that 32 bits count.
+__device__ __forceinline__ int64_t capacity(const PagesArgs &a) {
+  return min((int64_t)a.max_pages * a.page, (int64_t)0x7fffff00);
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -117,7 +122,7 @@ __global__ void __launch_bounds__(kBookThreads)
   int *upto = sh;  // [n_slot]
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t cap = (int64_t)a.max_pages * a.page;
+  const int64_t cap = capacity(a);
   int total = 0;
   for (int base = 0; base < a.n_slot; base += kBookThreads) {
     const int i = base + threadIdx.x;
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(kBookThreads)
   int *len = upto + n;           // [n] the source's length at the call, -1: refused
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t cap = (int64_t)a.max_pages * a.page;
+  const int64_t cap = capacity(a);
   for (int i = threadIdx.x; i < a.n_slot; i += kBookThreads) claim[i] = n;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kBookThreads)
@@ -329,8 +334,7 @@ __global__ void __launch_bounds__(256)
   if (s < 0 || s >= a.n_slot) return;
   if (threadIdx.x == 0) held = atomicExch(&a.n_ctx[s], 0);
   __syncthreads();
-  const int64_t most = (int64_t)a.max_pages * a.page;
-  const int n = pages_of((int)min((int64_t)max(held, 0), most), a.page);
+  const int n = pages_of((int)min((int64_t)max(held, 0), capacity(a)), a.page);
   int32_t *row = a.table + (int64_t)s * a.max_pages;
   for (int k = threadIdx.x; k < n; k += 256) {
     const int p = row[k];
