@@ -432,10 +432,10 @@ def pages_compact(cache, n_live=None, workspace=None):
     """Moves the pages in use to the front of the pool; returns their number (int32
     [1], device)."""
     dev = _device_of(cache)
-    n_live = n_live if n_live is not None else cache.n_ctx.new_empty(1)
     if workspace is None:
         workspace = torch.empty(core().w8a8_pages_compact_workspace_size(cache.n_pages),
                                 dtype=_U8, device=cache.device)
+    n_live = n_live if n_live is not None else cache.n_ctx.new_empty(1)
     check(core().w8a8_pages_compact(cache.ref, _here(n_live, _I32, dev, "n_live", 1),
                                     _here(workspace, _U8, dev, "workspace"), workspace.numel(),
                                     _raw_stream(dev)), "w8a8_pages_compact")
@@ -456,6 +456,8 @@ def _pool(t: torch.Tensor, like: torch.Tensor, dev: int, name: str) -> int:
 def _page_size(t: torch.Tensor, name: str) -> tuple[tuple, int, int]:
     """Shape of a pool's pages, their elements, and the pool's page stride."""
     shape, strides = t.shape, t.stride()
+    if t.is_contiguous() and len(shape) > 1 and shape[0] > 0:
+        return shape[1:], strides[0], strides[0]
     size = 1
     for n, s in zip(reversed(shape[1:]), reversed(strides[1:])):
         if n != 1 and s != size:

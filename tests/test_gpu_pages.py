@@ -542,3 +542,67 @@ def test_the_slot_cache_attention_agrees(cuda):
     A = np.stack([w[1][0] for w in want]).reshape(4, d)
     err = (slot.double() - page.double()).abs().cpu().numpy()
     assert (err <= (2.0 ** -8 * (2 * smax + 6)) * A).all()
+
+
+def test_a_serving_run(cuda):
+    """Two prompts of different lengths (a padded batch) through the packed QKV
+    projection into pages; three samples of each, decoded step by step behind the
+    first prompt's pages or their own; some given back, the pool compacted and
+    halved, and the rest decoded on. Every attention output against 64 bits over the
+    keys and values that the sequence has been given."""
+    d, H, page, T = 768, 12, 16, 70
+    g = torch.Generator(device=cuda).manual_seed(0)
+    W = torch.randint(-127, 128, (3 * d, d), generator=g, device=cuda, dtype=torch.int8)
+    sW = torch.full((3 * d,), 5e-4, device=cuda)
+    bias = torch.randn(3 * d, generator=g, device=cuda).bfloat16()
+    c = PageCache.empty(90, 8, 10, 1, H, page, cuda)
+    held = [[] for _ in range(8)]  # K, V rows of every slot
+
+    def project(rows):
+        Xq, sX = ops.per_token_quant(torch.randn(rows, d, generator=g, device=cuda).bfloat16())
+        Q, K, V = (torch.empty(rows, d, dtype=torch.bfloat16, device=cuda) for _ in range(3))
+        ops.linear_qkv(Xq, sX, W, sW, bias, Q, K, V, rows * d, rows)
+        return Q, K, V
+
+    def attend(Q, t, n_new, **kw):
+        out = torch.zeros_like(Q)
+        ops.attention_pages(Q, c, 0, H, T=t, n_new=i32(n_new), out=out, **kw)
+        q64 = Q.double().cpu().numpy().reshape(8, t, H, 64)
+        want = []
+        for s in range(8):
+            kv = [np.stack(x) if n_new[s] else np.zeros((0, H, 64))
+                  for x in (zip(*held[s]) if n_new[s] else ((), ()))]
+            want.append(po.attention(q64[s], *kv, n_new[s]))
+        check(out, want, t, H, n_new, before=0.0)
+
+    def step(t, n_new, **kw):
+        Q, K, V = project(8 * t)
+        pos0 = ops.pages_extend(c, i32(n_new))
+        assert (pos0.cpu().numpy() >= -1).all()
+        ops.pages_write(c, 0, K, V, pos0, T=t, n_new=i32(n_new))
+        k64, v64 = (x.double().cpu().numpy().reshape(8, t, H, 64) for x in (K, V))
+        for s in range(8):
+            held[s] += [(k64[s, i], v64[s, i]) for i in range(n_new[s])]
+        attend(Q, t, n_new, **kw)
+
+    step(T, [T, 41] + [0] * 6)
+    src, dst = [0, 0, 1, 1], [2, 4, 3, 7]
+    assert ops.pages_fork(c, i32(src), i32(dst)).tolist() == [0] * 4
+    for a, b in zip(src, dst):
+        held[b] = list(held[a])
+    for i in range(12):
+        step(1, [1, 1, 1, 1, 1, 0, 0, 1])
+    # behind the first prompt alone: the second's samples have left
+    ops.pages_free(c, i32([1, 3, 7]))
+    for s in (1, 3, 7):
+        held[s] = []
+    n_live = ops.pages_compact(c).item()
+    assert n_live == 4 + 3 * 2 and (c.refs[:4 + 6] > 0).all() and (c.refs[n_live:] == 0).all()
+    small = PageCache(c.K[:45].clone(), c.V[:45].clone(), c.table, c.n_ctx, c.refs[:45].clone())
+    c = small
+    for i in range(8):
+        step(1, [1, 0, 1, 0, 1, 0, 0, 0], shared_pages=c.table[2, :4].clone(), n_shared=64,
+             max_ctx=96)
+    step(30, [30, 0, 5, 0, 0, 0, 0, 0])  # two go on by more than a token
+    ops.pages_free(c, i32(range(8)))
+    assert c.refs.sum().item() == 0 and (c.table == -1).all() and (c.n_ctx == 0).all()
