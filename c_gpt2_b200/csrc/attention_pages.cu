@@ -1068,34 +1068,53 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
       const int at = blockIdx.x * kPairRows + g * kTileRows + r;
+      // Rows leave through this warp's share of its Q tile, which no product reads any more, 32
+      // dims at a time: a lane's row in, eight lanes a row out, four lines a store (a lane a row
+      // would touch 32 lines with each).
+      uint8_t *buf = sQ + g * kTcTile + qd * 32 * 128;
+      const int sub = lane >> 3, chunk = lane & 7;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        float x[32];
+        {
+          uint32_t o[32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[16], o1[16];
-        if (mine > 0) {
-          tmem_ld_32x32b_x16(trow + kColO + 16 * c, o);
-        } else {
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
+          if (mine > 0) tmem_ld_32x32b_x32(trow + kColO + 32 * half, o);
+          tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0u;
+          for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(o[k]);
         }
-        if (second) tmem_ld_32x32b_x16(trow + kColGroup + kColO + 16 * c, o1);
-        tmem_ld_wait();
-        float x[16];
+        if (second) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(trow + kColGroup + kColO + 32 * half, o);
+          tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          x[k] = __uint_as_float(o[k]);
-          if (second) x[k] = f0 * x[k] + f1 * __uint_as_float(o1[k]);
+          for (int k = 0; k < 32; ++k) x[k] = f0 * x[k] + f1 * __uint_as_float(o[k]);
         }
-        if (row.m >= 0) {
+        const float scale = a.direct ? inv : 1.0f;
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<float4 *>(buf + lane * 128 + ((k ^ (lane & 7)) * 16)) =
+              make_float4(x[4 * k] * scale, x[4 * k + 1] * scale, x[4 * k + 2] * scale,
+                          x[4 * k + 3] * scale);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int q = 4 * i + sub;
+          const float4 y =
+              *reinterpret_cast<const float4 *>(buf + q * 128 + ((chunk ^ (q & 7)) * 16));
+          const int m = __shfl_sync(~0u, row.m, q), h = __shfl_sync(~0u, row.h, q);
+          if (m < 0) continue;
+          const int d0 = 32 * half + 4 * chunk;
           if (a.direct) {
             uint32_t *dst =
-                reinterpret_cast<uint32_t *>(a.O + (int64_t)row.m * a.ldo + row.h * kPageHd + 16 * c);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k] = pack_bf2(x[2 * k] * inv, x[2 * k + 1] * inv);
+                reinterpret_cast<uint32_t *>(a.O + (int64_t)m * a.ldo + h * kPageHd + d0);
+            dst[0] = pack_bf2(y.x, y.y);
+            dst[1] = pack_bf2(y.z, y.w);
           } else {
-            float4 *dst = reinterpret_cast<float4 *>(a.Op + (int64_t)at * kPageHd + 16 * c);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              dst[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+            *reinterpret_cast<float4 *>(a.Op + (int64_t)(at - lane + q) * kPageHd + d0) = y;
           }
         }
       }
