@@ -470,6 +470,43 @@ def test_another_stream_and_captured_graphs(cuda):
     assert ca.refs.sum().item() == 4 * 5 and ca.table[:, :2].unique().numel() == 2
 
 
+@pytest.mark.parametrize("T,n_shared", [(1, 64), (1, 0), (3, 320), (90, 32)])
+def test_strided_rows_and_fewer_sequences_than_slots(cuda, T, n_shared):
+    """Q in a packed [Q | K | V] row, an output with padded rows, and the first three
+    of five slots: the same bits as contiguous rows, and nothing beside them written."""
+    tails = [T + 5, T, T + 200, T + 1, T + 2]
+    c, Q, shared, want = build(cuda, 5, T, 4, 2, 32, n_shared, tails, [T] * 5, 7)
+    kw = dict(T=T, max_ctx=n_shared + max(tails), shared_pages=shared, n_shared=n_shared)
+    plain = ops.attention_pages(Q[:3 * T].contiguous(), c, 1, 4, **kw)
+    check(plain, want[:3], T, 4, [T] * 3)
+    packed = torch.full((3 * T, 520), 3.0, dtype=torch.bfloat16, device=cuda)
+    packed[:, 8:264] = Q[:3 * T]
+    wide = torch.full((3 * T, 262), 7.0, dtype=torch.bfloat16, device=cuda)
+    ops.attention_pages(packed[:, 8:264], c, 1, 4, out=wide[:, 2:258], **kw)
+    assert torch.equal(wide[:, 2:258], plain)
+    assert (wide[:, :2] == 7).all() and (wide[:, 258:] == 7).all()
+
+
+def test_two_caches_on_two_streams(cuda):
+    """Calls in flight together, each on its own cache, stream and workspace."""
+    made = [build(cuda, n, T, 8, 8, 64, P, [T + 7 * i for i in range(n)], [T] * n, n)
+            for n, T, P in ((300, 1, 1728), (3, 90, 128), (40, 1, 64))]
+    args = [(c, Q, dict(T=T, max_ctx=P + T + 7 * n, shared_pages=s, n_shared=P))
+            for (c, Q, s, _), (n, T, P) in zip(made, ((300, 1, 1728), (3, 90, 128), (40, 1, 64)))]
+    alone = [ops.attention_pages(Q, c, 1, 8, **kw) for c, Q, kw in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    outs = [[], [], []]
+    for _ in range(20):
+        for i, (c, Q, kw) in enumerate(args):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(ops.attention_pages(Q, c, 1, 8, **kw))
+    torch.cuda.synchronize()
+    for i in range(3):
+        for o in outs[i]:
+            assert torch.equal(o, alone[i])
+
+
 def test_front_end_refusals(cuda):
     c, _ = make(cuda, 8, 2, 4)
     f = dict(device=cuda)
@@ -497,7 +534,10 @@ def test_front_end_refusals(cuda):
     bad = [dict(layer=2), dict(layer=-1), dict(n_head=4, Q=torch.zeros(2, 256, dtype=torch.bfloat16, **f)),
            dict(max_ctx=0), dict(n_shared=8, shared_pages=one), dict(workspace=ws, max_ctx=64),
            dict(n_shared=32, max_ctx=16, shared_pages=one),
-           dict(Q=torch.zeros(3, 192, dtype=torch.bfloat16, **f))]
+           dict(Q=torch.zeros(3, 192, dtype=torch.bfloat16, **f)),
+           dict(Q=torch.zeros(2, 200, dtype=torch.bfloat16, **f)[:, 4:196]),   # 8-byte aligned
+           dict(Q=torch.zeros(2, 196, dtype=torch.bfloat16, **f)[:, :192]),    # ldq % 8
+           dict(out=torch.zeros(2, 193, dtype=torch.bfloat16, **f)[:, :192])]  # odd ldo
     for kw in bad:
         kw = dict(dict(Q=Q, layer=0, n_head=3), **kw)
         with pytest.raises(_lib.W8A8Error) as e:
