@@ -4,15 +4,19 @@
 //
 // formed in one pass over the keys (running maximum and sum; base-2
 // exponentials of scores scaled by log2(e) / 8), with fp32 scores, maxima, sums
-// and accumulators. The weights are rounded to bf16 for the tensor cores: at
-// most half a step, 2^-9 of each weight and of either sign, below the rounding
-// of the output itself.
+// and accumulators. The weights are rounded to bf16 for the tensor cores: half a
+// step at most, 2^-8 of a weight and of either sign, which an average over keys
+// shrinks below the rounding of the output; their sum is taken before it.
 //
-// The key axis of a row is cut into the shared prefix and the sequence's own
-// tail, and each of those into chunks; every (rows, chunk) pair is an item of
-// work that leaves (m, sum, unnormalised O) in the workspace, and a last kernel
-// joins a row's items. The prefix items take rows of ALL sequences, so the
-// shared pages are read once for 16 rows, not once a sequence.
+// Rows and keys are cut up so that shared keys are read once for many rows:
+//   tensor-core items (tcgen05)  up to 256 rows: of all sequences over the shared
+//                                prefix, or of one over prefix and tail
+//   16-row groups (mma.sync)     the few rows of one sequence and key head over
+//                                its tail, or over a prefix that few rows share
+// Both leave parts (maximum, sum, unnormalised O) of their rows in the workspace,
+// which a last kernel joins; a call whose every row is one item's or one group's
+// writes O at once. make_plan has the choice. Lengths are known on the device
+// only, so the kernels cut the keys themselves.
 #include "common.cuh"
 #include "kernels.cuh"
 #include "runtime.cuh"
@@ -490,10 +494,14 @@ __device__ __forceinline__ void mma_stage(MmaState &w, uint32_t kb, uint32_t vb,
 // ---------------------------------------------------------------------------
 // Items of 16 rows on mma.sync, a warp each: for the tails, whose row tile holds
 // the few rows of one sequence and key head, and for a prefix that few rows
-// share. Bound by HBM in principle (23 bytes a cycle and SM: 64 keys of a head,
-// 16 KB, in 700 cycles), by issue and latency in practice. So the warps work
-// alone, with no barrier between them, each with two 64-key stages that it
-// fills itself by TMA (128-byte swizzle), one ahead, across the ends of items.
+// share. Bound by HBM: 64 keys of a head, 16 KB, in 700 cycles of an SM at the
+// copy rate. The warps work alone, with no barrier between them, each with two
+// 64-key stages that it fills itself by TMA (128-byte swizzle), one ahead, across
+// the ends of items (four warps with three stages: 31 us where six with two take
+// 25.5, seven 24.5). Measured, 64 sequences of 20 heads, nothing shared: 5.4 TB/s
+// with up to 4096 positions each (683 MB, 125 us; without the arithmetic 118), but
+// 29 us with up to 512 (85 MB): some 4 us until the first keys arrive, 4 for the
+// join, and SMs that get their bytes up to a fifth later than the average.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(kMmaWarps * 32, 1)
     attention_pages_mma_kernel(const __grid_constant__ CUtensorMap tmK,
@@ -697,8 +705,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
 // the exponentials of this one run, and the groups' MMAs overlap each other's
 // softmax. A single tile (the last rows, or few of them) is worked on by both
 // groups, a block each in turn, which are joined at the end.
-// Bound by the exponentials: 128 x 128 of them at 16 a cycle are 1024 cycles,
-// the two products of a tile 512.
+// Bound by the exponentials and what goes with them: a pair of tiles takes some
+// 2900-3200 cycles a block; 2 x 128 x 128 exponentials alone take 2400 (9.4 cycles a
+// warp's instruction, measured), the MMAs 1530. Tried and slower: a fourth or more
+// of the exponentials as polynomials on the multiply-add units (77 us with 1/8, 83
+// with 3/8, as without: 77, of which this kernel is 47); two warps a quarter-tile,
+// half a row each (67 against 49 us); scores read from TMEM twice in rolled loops
+// (58 against 47); no turns (52 against 47). A CTA spends some 14000 cycles outside
+// its blocks (plan, rows, Q, first scores, output), which across_of counts.
 // ---------------------------------------------------------------------------
 namespace {
 

@@ -319,7 +319,8 @@ int w8a8_pages_free(const w8a8_pages *c, const int32_t *slots, int n, void *stre
 
 /* Moves the pages in use to the front of the pool: with n_live[0] of them (device,
  * written), the j-th at index >= n_live goes to the j-th free index below, and
- * the table follows. Pages from n_live on are free afterwards.
+ * the table follows (indices kept elsewhere, a list of shared pages say, do not).
+ * Pages from n_live on are free afterwards.
  * workspace: w8a8_pages_compact_workspace_size(n_pages) bytes, any contents. */
 size_t w8a8_pages_compact_workspace_size(int n_pages);
 int w8a8_pages_compact(const w8a8_pages *c, int32_t *n_live, void *workspace,
@@ -349,9 +350,13 @@ int w8a8_pages_copy(const gpt2_bf16_t *Ksrc, const gpt2_bf16_t *Vsrc, int64_t sr
  * prompt, any one's table row. Rows of pages that no query attends may hold
  * anything; a value that is not finite at a position that some query attends
  * may reach every query of the call that shares its key head.
- * max_ctx bounds every n_ctx[b]. The workspace (any contents) is sized with
- * w8a8_attention_pages_workspace_size; 16-byte aligned Q, ldq % 8 == 0, O
- * 4-byte aligned, ldo even; n_head % n_kv_head == 0, head_dim 64. */
+ * max_ctx bounds every n_ctx[b] (<= 2^30). The workspace (any contents; calls
+ * that share one must not overlap on the GPU) is sized with
+ * w8a8_attention_pages_workspace_size, 0 for sizes that are refused; 16-byte
+ * aligned Q and workspace, ldq % 8 == 0, O 4-byte aligned, ldo even;
+ * n_head % n_kv_head == 0, head_dim 64, n_seq*T*n_head <= 2^30. Calls of more
+ * than 2^31 (16 rows x 64 keys) pieces are W8A8_ERR_UNSUPPORTED. The outcome does
+ * not depend on the order in which anything runs. */
 size_t w8a8_attention_pages_workspace_size(int n_seq, int T, int n_head, int n_kv_head,
                                            int max_ctx, int n_shared);
 int w8a8_attention_pages(const w8a8_pages *c, int layer, const gpt2_bf16_t *Q, int64_t ldq,
