@@ -338,6 +338,20 @@ def test_keys_nobody_sees_may_hold_anything(cuda, n_seq, T):
         assert torch.equal(outs[0].view(torch.int16), o.view(torch.int16))
 
 
+@pytest.mark.parametrize("T,n_shared", [(3, 0), (3, 320), (70, 32), (300, 0)])
+def test_a_key_that_is_not_a_number(cuda, T, n_shared):
+    """NaN in the newest position's key reaches the row that sees it and no other."""
+    tails = [T + 40, T + 3]
+    c, Q, shared, _ = build(cuda, 2, T, 4, 2, 32, n_shared, tails, [T] * 2, 11)
+    kw = dict(T=T, max_ctx=n_shared + T + 40, shared_pages=shared, n_shared=n_shared)
+    want = ops.attention_pages(Q, c, 1, 4, **kw)
+    last = n_shared + tails[0] - 1
+    c.K[c.table[0, last // 32].item(), 1, :, last % 32] = float("nan")
+    got = ops.attention_pages(Q, c, 1, 4, **kw)
+    rows = [r for r in range(2 * T) if r != T - 1]
+    assert torch.equal(got[rows], want[rows]) and got[T - 1].isnan().all()
+
+
 @pytest.mark.parametrize("n_seq,T,n_shared", [(2, 1, 512), (64, 1, 512), (2, 130, 512), (3, 1, 0)])
 def test_large_scores(cuda, n_seq, T, n_shared):
     """Scores of some hundreds, growing along the keys and falling: the running
