@@ -36,7 +36,7 @@ constexpr int kErrWaitFull = 0x1602;
 constexpr int kStageKeys = 64;
 constexpr int kStages = 2;                         // of each warp
 constexpr uint32_t kTileBytes = kStageKeys * 128;  // keys or values of a stage
-constexpr int kMmaWarps = 7;                       // one CTA an SM, a warp an item
+constexpr int kMmaWarps = 7;                       // of a CTA, one an SM
 constexpr int kRows = 16;                          // query rows of an item
 // A prefix of more 16-row stages than this goes to the tensor-core kernel, if it takes several
 // row tiles. That kernel has a fixed cost of some 8 us; the 16-row kernel, whose re-reads hit
@@ -68,6 +68,7 @@ constexpr int kTcKeys = 128;                     // and keys of a block
 // packed, in pairs of tiles and perhaps a last single one, the keys of a pair in s2 chunks of
 // c2, a single tile's in s1 of c1. A CTA's time goes by its blocks, and a single tile's take
 // half as long, so its chunks are twice as long.
+constexpr int kMostCost = 1 << 25;
 struct Across {
   int rows, pairs, s2, c2, s1, c1;  // s1 = 0: no single tile
   int cost;                         // rounds of CTAs times blocks of one
@@ -88,8 +89,8 @@ __host__ __device__ inline Across across_of(int rows, int n_kv, int n_shared, in
   p.s2 = p.pairs ? (blocks + b2 - 1) / b2 : 0;
   p.s1 = single ? (blocks + b1 - 1) / b1 : 0;
   const int items = n_kv * (p.pairs * p.s2 + p.s1);
-  p.cost = (items + kSms - 1) / kSms * (p.pairs ? b2 + 3 : (b1 + 1) / 2 + 3);
-  if (splits > 1 && items > max_items) p.cost = 0x7fffffff;
+  const int64_t cost = (int64_t)((items + kSms - 1) / kSms) * (p.pairs ? b2 + 3 : (b1 + 1) / 2 + 3);
+  p.cost = cost < kMostCost && (splits == 1 || items <= max_items) ? (int)cost : kMostCost;
   return p;
 }
 
@@ -108,8 +109,8 @@ struct ApArgs {
   int base;            // where a sequence's groups begin: n_shared, or 0 if nothing is shared out
   int whole;           // stages given to every sequence's groups, none split; 0: as many as it has
   // tensor-core items: rows of one sequence over all its keys, [pairs][n_seq][n_kv][splits]
-  // of `chunk` keys; or of all sequences over the prefix, as
-  // `across` has them (all T rows of a sequence hold a query), or as plan_across finds
+  // of `chunk` keys; or of all sequences over the prefix, as `across` has them (if every row
+  // holds a query) or plan_across finds them
   int by_seq, pairs, splits, chunk;
   Across across;
   int tc;              // CTAs of the tensor-core kernel
@@ -140,29 +141,7 @@ struct Row {
   int m;  // token row, -1: none
   int h, end;
 };
-// Row R of the (m, g) rows of sequence `seq` (-1: of all) and one key head.
-__device__ __forceinline__ Row get_row(const ApArgs &a, int seq, int kvh, int R) {
-  Row w;
-  w.m = quot(R, a.by_g);
-  w.h = kvh * a.g + (R - w.m * a.g);
-  int b = seq, t = w.m;
-  if (b < 0) {
-    b = quot(w.m, a.by_T);
-    t = w.m - b * a.T;
-  } else {
-    w.m += b * a.T;
-  }
-  w.end = 0;
-  if (b >= a.n_seq) {
-    w.m = -1;
-    return w;
-  }
-  const int nn = seq_new(a, b);
-  if (t >= nn) w.m = -1;
-  else w.end = seq_len(a, b) - nn + t + 1;
-  return w;
-}
-
+// (volatile: the exponentials stay between the barriers of a turn at them)
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -379,14 +358,20 @@ __device__ __forceinline__ Item walk_next(const ApArgs &a, Walk &w, int lane) {
   return it;
 }
 
-// Row R of an item's; for the rows of one sequence nothing is read.
+// Row R of an item's (m, g) rows; for those of one sequence nothing is read.
 __device__ __forceinline__ Row get_row(const ApArgs &a, const Item &it, int R) {
-  if (it.b < 0) return get_row(a, -1, it.kvh, R);
   Row w;
-  const int t = quot(R, a.by_g);
-  w.h = it.kvh * a.g + (R - t * a.g);
-  w.m = t < it.nn ? it.b * a.T + t : -1;
-  w.end = t < it.nn ? it.n_valid - it.nn + t + 1 : 0;
+  const int j = quot(R, a.by_g);
+  w.h = it.kvh * a.g + (R - j * a.g);
+  int b = it.b, t = j, nn = it.nn, len = it.n_valid;
+  if (b < 0) {
+    b = quot(j, a.by_T);
+    t = j - b * a.T;
+    nn = b < a.n_seq ? seq_new(a, b) : 0;
+    len = b < a.n_seq ? seq_len(a, b) : 0;
+  }
+  w.m = t < nn ? b * a.T + t : -1;
+  w.end = t < nn ? len - nn + t + 1 : 0;
   return w;
 }
 
@@ -541,22 +526,22 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
   const bool act = lane < 2 * boxes, is_v = lane >= boxes;
   const int bx = is_v ? lane - boxes : lane;
   Walk ahead = walk;  // of the loads
-  Item it;
-  int stage = 0, stages = 0;
+  Item coming;        // the item that is being loaded
+  int at_stage = 0, of_stages = 0;
   auto next_item = [&]() {  // one with keys
-    stage = stages = 0;
-    while (stages == 0 && ahead.left > 0) {
-      it = walk_next(a, ahead, lane);
-      stages = item_stages(it);
+    at_stage = of_stages = 0;
+    while (of_stages == 0 && ahead.left > 0) {
+      coming = walk_next(a, ahead, lane);
+      of_stages = item_stages(coming);
     }
   };
   auto entry = [&]() -> int {  // page of this lane's box, n_pages: reads as zeros
-    const int pos = it.k0 + stage * kStageKeys + bx * box;
-    if (!act || stages == 0 || pos >= it.k1) return a.n_pages;
+    const int pos = coming.k0 + at_stage * kStageKeys + bx * box;
+    if (!act || of_stages == 0 || pos >= coming.k1) return a.n_pages;
     const int k = pos >> a.page_shift;
     int p = -1;
     if (pos < a.n_shared) p = a.shared[k];
-    else if (k < a.max_pages) p = a.table[(int64_t)it.b * a.max_pages + k];
+    else if (k < a.max_pages) p = a.table[(int64_t)coming.b * a.max_pages + k];
     if (p < 0 || p >= a.n_pages) {
       report_error(a.err, kErrEntry);
       p = a.n_pages;
@@ -567,18 +552,18 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
   int page = entry();
   uint32_t loaded = 0;
   auto load = [&]() {
-    if (stages == 0) return;
+    if (of_stages == 0) return;
     const int st = loaded % kStages;
     if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * kTileBytes);
     __syncwarp();
     if (act) {
-      const int pos = it.k0 + stage * kStageKeys + bx * box;
-      const int y = (it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+      const int pos = coming.k0 + at_stage * kStageKeys + bx * box;
+      const int y = (coming.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
       tma_load_3d(ring + (st * 2 + is_v) * kTileBytes + bx * box * 128, is_v ? &tmV : &tmK,
                   &full[st], 0, y, page);
     }
     ++loaded;
-    if (++stage == stages) next_item();
+    if (++at_stage == of_stages) next_item();
     page = entry();
   };
 #pragma unroll 1
@@ -744,6 +729,7 @@ struct TcItem {
   int split, splits;  // of the rows' items over their keys
 };
 
+// The items over the prefix; how many rows of a padded batch hold a query is known here only.
 __device__ __forceinline__ Across plan_across(const ApArgs &a, int lane) {
   if (!a.n_new) return a.across;
   int valid = 0;
@@ -752,7 +738,7 @@ __device__ __forceinline__ Across plan_across(const ApArgs &a, int lane) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) valid += __shfl_xor_sync(~0u, valid, d);
   Across p = across_of(valid * a.g, a.n_kv, a.n_shared, lane + 1, a.tc);
-  int best = min(p.cost, 1 << 25) << 5 | lane;  // a lane a choice
+  int best = p.cost << 5 | lane;  // a lane a choice
 #pragma unroll
   for (int d = 16; d; d >>= 1) best = min(best, __shfl_xor_sync(~0u, best, d));
   p.c2 = __shfl_sync(~0u, p.c2, best & 31);
@@ -907,7 +893,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile int *abort_flag = &ctl->abort_flag;
 
   if (warp < 8) {
-    reg_alloc<208>();
+    reg_alloc<208>();  // 256 x 208 + 128 x 88 are the launch's 384 x 168
     // ---------------- softmax ----------------
     const int g = warp >> 2, qd = warp & 3;
     const int r = qd * 32 + lane;  // TMEM lane
@@ -1403,7 +1389,7 @@ int make_plan(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared,
       if (tc_grid < 2 * kSms) tc_grid = 2 * kSms;
     } else if (a_stages <= 4 && (n_shared == 0 || groups <= kSms * kMmaWarps)) {
       // short sequences, a group a warp if they share anything: whole groups, which read what is
-      // shared for themselves, and no join (2 sequences of 96, 64 shared: 14.0 -> 11.4 us a call)
+      // shared for themselves, and no join (2 sequences of 96, 64 shared: 14.0 -> 10.4 us a call)
       p.base = 0;
       p.whole = (int)a_stages;
       p.direct = true;
