@@ -442,28 +442,28 @@ def pages_compact(cache, n_live=None, workspace=None):
     return n_live
 
 
-def _pool(t: torch.Tensor, like: torch.Tensor, dev: int, name: str) -> int:
-    """Address of a bf16 pool of contiguous pages shaped and strided as `like`."""
-    if t.dtype != _BF16:
-        raise TypeError(f"{name}: expected {_BF16}, got {t.dtype}")
-    if t.get_device() != dev:
-        raise ValueError(f"{name}: expected a tensor on the current CUDA device")
-    if t is not like and (t.shape != like.shape or t.stride() != like.stride()):
-        raise ValueError(f"{name}: expected shape and strides of its pair")
-    return t.data_ptr()
-
-
-def _page_size(t: torch.Tensor, name: str) -> tuple[tuple, int, int]:
-    """Shape of a pool's pages, their elements, and the pool's page stride."""
-    shape, strides = t.shape, t.stride()
-    if t.is_contiguous() and len(shape) > 1 and shape[0] > 0:
-        return shape[1:], strides[0], strides[0]
-    size = 1
-    for n, s in zip(reversed(shape[1:]), reversed(strides[1:])):
-        if n != 1 and s != size:
-            raise ValueError(f"{name}: expected contiguous pages")
-        size *= n
-    return shape[1:], size, strides[0] if shape[0] > 1 else size
+def _pools(K: torch.Tensor, V: torch.Tensor, dev: int, names: str):
+    """Addresses of a pair of bf16 pools of contiguous pages, their shape, the elements
+    of a page and the page stride."""
+    if K.dtype != _BF16 or V.dtype != _BF16:
+        raise TypeError(f"{names}: expected {_BF16}, got {K.dtype}, {V.dtype}")
+    if K.get_device() != dev or V.get_device() != dev:
+        raise ValueError(f"{names}: expected tensors on the current CUDA device")
+    shape = K.shape
+    if V.shape != shape or len(shape) < 2:
+        raise ValueError(f"{names}: expected pools of one shape, pages first")
+    if K.is_contiguous() and V.is_contiguous():
+        size = stride = K.stride(0)
+    else:
+        strides, size = K.stride(), 1
+        for n, s in zip(reversed(shape[1:]), reversed(strides[1:])):
+            if n != 1 and s != size:
+                raise ValueError(f"{names}: expected contiguous pages")
+            size *= n
+        if V.stride() != strides:
+            raise ValueError(f"{names}: expected equally strided pools")
+        stride = strides[0] if shape[0] > 1 else size
+    return K.data_ptr(), V.data_ptr(), shape, size, stride
 
 
 def pages_copy(Ksrc, Vsrc, src, Kdst, Vdst, dst):
@@ -471,15 +471,13 @@ def pages_copy(Ksrc, Vsrc, src, Kdst, Vdst, dst):
     dimension counts pages). The dst pages are distinct, and none is a source."""
     dev = _current(Ksrc.get_device(), "Ksrc")
     n = src.numel()
-    page, size, ss = _page_size(Ksrc, "Ksrc")
-    page_dst, _, ds = _page_size(Kdst, "Kdst")
-    if page != page_dst:
-        raise ValueError(f"Kdst: expected pages of {tuple(page)}, got {tuple(page_dst)}")
-    check(core().w8a8_pages_copy(
-        _pool(Ksrc, Ksrc, dev, "Ksrc"), _pool(Vsrc, Ksrc, dev, "Vsrc"), ss, Ksrc.shape[0],
-        _pool(Kdst, Kdst, dev, "Kdst"), _pool(Vdst, Kdst, dev, "Vdst"), ds, Kdst.shape[0], size,
-        _here(src, _I32, dev, "src", n), _here(dst, _I32, dev, "dst", n), n, _raw_stream(dev)),
-        "w8a8_pages_copy")
+    ks, vs, shape_s, size, stride_s = _pools(Ksrc, Vsrc, dev, "Ksrc, Vsrc")
+    kd, vd, shape_d, _, stride_d = _pools(Kdst, Vdst, dev, "Kdst, Vdst")
+    if shape_s[1:] != shape_d[1:]:
+        raise ValueError(f"Kdst: expected pages of {tuple(shape_s[1:])}, got {tuple(shape_d[1:])}")
+    check(core().w8a8_pages_copy(ks, vs, stride_s, shape_s[0], kd, vd, stride_d, shape_d[0], size,
+                                 _here(src, _I32, dev, "src", n), _here(dst, _I32, dev, "dst", n),
+                                 n, _raw_stream(dev)), "w8a8_pages_copy")
 
 
 @functools.lru_cache(maxsize=4096)

@@ -563,6 +563,15 @@ def test_front_end_refusals(cuda):
         ops.pages_write(c, 0, Q.view(-1)[4:4 + 192].view(1, 192), Q[:1], i32([0]))
     with pytest.raises(_lib.W8A8Error):
         ops.pages_compact(c, workspace=ws)
+    K, V = c.K, c.V
+    for bad, err in [((K.float(), V, one, K, V, one), TypeError), ((K, V.float(), one, K, V, one), TypeError),
+                     ((K, V, one, K[:, :1], V[:, :1], one), ValueError),       # other pages
+                     ((K, V[:4], one, K, V, one), ValueError), ((K, V, one, K, V, i32([1])), ValueError),
+                     ((K[..., ::2], V[..., ::2], one, K, V, one), ValueError),  # scattered pages
+                     ((K, V[::2], one, K, V, one), ValueError), ((K, V.cpu(), one, K, V, one), ValueError),
+                     ((K, V, one.long(), K, V, one), TypeError)]:
+        with pytest.raises(err):
+            ops.pages_copy(*bad)
     assert c.n_ctx.tolist() == [0, 0]
 
 
