@@ -121,7 +121,7 @@ struct ApArgs {
   // Parts of rows: 256 of each tensor-core item; then, of the 16-row groups, one a row over the
   // prefix (at part_p) and one over the tail (part_t); and, of groups that several warps share,
   // [warps][2][16] (part_f): a warp's rows of the group it joined, and of the one it began.
-  int64_t part_p, part_t, part_f;
+  int64_t part_p, part_t, part_f, parts;
   float *Op;           // [part][64]
   float2 *ml;          // [part] maximum (base 2), sum
   // [3][rows]: first part (tensor-core items) or first warp of the row's parts over the prefix,
@@ -1267,16 +1267,17 @@ __global__ void __launch_bounds__(256)
   const int first = a.shares[row], n_first = a.shares[a.rows + row];
   const int tail_word = a.shares[2 * a.rows + row];
   if (t >= seq_new(a, b)) return;
-  const int n1 = a.tc || a.p_stages ? n_first : 0;
+  const int n1 = a.tc || a.p_stages ? min(max(n_first, 0), 0xffff) : 0;
   const int tail = !a.by_seq && tail_stages(a, seq_len(a, b)) > 0 ? tail_word : 0;
   const int n2 = n1 + (tail & 0xffff);
   const int gi = h - quot(h, a.by_g) * a.g;
   const int R = (m * a.g + gi) & (kRows - 1), Rt = (t * a.g + gi) & (kRows - 1);  // in their tiles
   // parts: of the prefix (or of all keys), then of the tail
   auto part = [&](int i) -> int64_t {
-    if (i < n1 && a.tc) return first + i * kPairRows;
+    if (i < n1 && a.tc) return (int64_t)first + i * kPairRows;
     if (i < n1)
-      return n1 == 1 ? a.part_p + row : a.part_f + ((first + i) * 2 + (i == 0)) * kRows + R;
+      return n1 == 1 ? a.part_p + row
+                     : a.part_f + (((int64_t)first + i) * 2 + (i == 0)) * kRows + R;
     i -= n1;
     return (tail & 0xffff) == 1 ? a.part_t + row
                                 : a.part_f + (((tail >> 16) + i) * 2 + (i == 0)) * kRows + Rt;
@@ -1287,8 +1288,10 @@ __global__ void __launch_bounds__(256)
     float4 x[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool live = i0 + i < n2;
-      const int64_t at = live ? part(i0 + i) : 0;
+      int64_t at = i0 + i < n2 ? part(i0 + i) : -1;
+      // (words that a kernel which gave up on a wait has not written may hold anything)
+      const bool live = at >= 0 && at < a.parts;
+      if (!live) at = 0;
       const float4 *src = reinterpret_cast<const float4 *>(a.Op + at * kPageHd + d0);
       v[i] = live ? a.ml[at] : make_float2(-INFINITY, 0.0f);
       x[i][0] = live ? src[0] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1493,6 +1496,7 @@ int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStrea
   a.part_p = p.part_p;
   a.part_t = p.part_t;
   a.part_f = p.part_f;
+  a.parts = p.parts;
   a.Op = reinterpret_cast<float *>(q.ws);
   a.ml = reinterpret_cast<float2 *>(a.Op + p.parts * kPageHd);
   a.shares = reinterpret_cast<int *>(a.ml + p.parts);
