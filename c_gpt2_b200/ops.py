@@ -491,12 +491,14 @@ def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shar
     b*T + t of Q [n_seq*T, n_head*64] for t < n_new[b] (default: all T; the other
     rows of the output are left as they were). The first n_shared positions are
     read, once for the batch, from shared_pages (int32, device); max_ctx (default:
-    the table's) bounds every length."""
+    what the table holds) bounds every length."""
     dev = _device_of(cache)
     d = n_head * 64
     n_seq = Q.shape[0] // T if T > 0 else 0
     if max_ctx is None:
-        max_ctx = cache.max_pages * cache.page
+        max_ctx = min(cache.max_pages * cache.page, 1 << 30)
+    if max_ctx > 1 << 30 or n_shared > 1 << 30:  # (32 bits further down)
+        raise ValueError("max_ctx, n_shared: expected at most 2^30 positions")
     if n_shared > 0 and (shared_pages is None or shared_pages.numel() * cache.page < n_shared):
         raise ValueError("shared_pages: expected a page for every n_shared position")
     q, ldq = _rows(Q, n_seq * T, d, dev, "Q")

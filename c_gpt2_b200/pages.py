@@ -37,7 +37,7 @@ class PageCache:
                 raise TypeError(f"{name}: expected {torch.int32}, got {t.dtype}")
             if not t.is_contiguous():
                 raise ValueError(f"{name}: expected a contiguous tensor")
-        if K.dim() != 5 or K.shape != V.shape or K.shape[4] != HEAD_DIM:
+        if K.dim() != 5 or K.shape != V.shape or K.shape[4] != HEAD_DIM or K.shape[0] == 0:
             raise ValueError("K, V: expected [n_pages, n_layer, n_kv_head, page, 64] each")
         if K.stride() != V.stride() or not K[0].is_contiguous():
             raise ValueError("K, V: expected contiguous pages, equally strided")

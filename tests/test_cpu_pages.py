@@ -92,6 +92,9 @@ def _cpu_cache(**kw):
     (dict(table=torch.zeros(3, 4, dtype=torch.int32)), ValueError),
     (dict(n_ctx=torch.zeros(2)), TypeError),
     (dict(refs=torch.zeros(7, dtype=torch.int32)), ValueError),
+    (dict(K=torch.zeros(0, 2, 3, 16, 64, dtype=torch.bfloat16),
+          V=torch.zeros(0, 2, 3, 16, 64, dtype=torch.bfloat16),
+          refs=torch.zeros(0, dtype=torch.int32)), ValueError),
 ])
 def test_page_cache_refuses_tensors(bad, err):
     with pytest.raises(err):

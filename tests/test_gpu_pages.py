@@ -544,6 +544,9 @@ def test_front_end_refusals(cuda):
         ops.attention_pages(Q, c, 0, 3, n_shared=16)
     with pytest.raises(TypeError):
         ops.attention_pages(Q.float(), c, 0, 3)
+    for n in ((1 << 30) + 1, (1 << 32) + 16):  # the second is 16 in 32 bits
+        with pytest.raises(ValueError):
+            ops.attention_pages(Q, c, 0, 3, max_ctx=n)
     ws = torch.empty(8, dtype=torch.uint8, **f)
     bad = [dict(layer=2), dict(layer=-1), dict(n_head=4, Q=torch.zeros(2, 256, dtype=torch.bfloat16, **f)),
            dict(max_ctx=0), dict(n_shared=8, shared_pages=one), dict(workspace=ws, max_ctx=64),
