@@ -844,8 +844,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     attention_pages_tc_kernel(const __grid_constant__ CUtensorMap tmK,
                               const __grid_constant__ CUtensorMap tmV,
                               const __grid_constant__ ApArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  // (an address known when this is compiled: no register holds it; 96 rows of 32 heads behind
+  // 32832 keys: 77.5 -> 75.9 us a call)
+  extern __shared__ __align__(1024) uint8_t smem_tc[];
+  uint8_t *smem = smem_tc;
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) report_error(a.err, kErrTc + 12);
+    return;
+  }
   uint8_t *sQ = smem;                       // [2] tiles
   uint8_t *sKV = smem + 2 * kTcTile;        // [stages] K, V
   TcCtl *ctl = reinterpret_cast<TcCtl *>(sKV + kTcStages * 2 * kTcTile);

@@ -280,6 +280,11 @@ CASES = [
     (5, 40, 12, 4, 32, 1760, [40, 90, -1, 41, 60]),
     (70, 5, 7, 7, 16, 2000, [5 + i % 9 if i % 7 else -1 for i in range(70)]),
     (4, 100, 6, 6, 32, 2848, [100, 101, 150, 130]),
+    # short prefixes of many rows, whose last block the prefix ends inside
+    (260, 7, 20, 20, 16, 80, [7 + i % 9 for i in range(260)]),
+    (300, 7, 32, 32, 16, 48, [7 + i % 40 for i in range(300)]),
+    (130, 8, 20, 20, 32, 320, [8 + i % 30 if i % 5 else -1 for i in range(130)]),
+    (130, 8, 20, 20, 64, 384, [8 + i % 30 for i in range(130)]),
     # more keys of the sequences' own than shared, and rows enough: prefix and tail in one item
     (2, 70, 4, 2, 32, 64, [70, 2300]),
     (3, 300, 2, 1, 64, 128, [300, 1500, 400]),
