@@ -670,7 +670,10 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
       }
     }
   }
-  if (a.behind) pdl_wait();  // this kernel's end is to mean the other's too
+  // This kernel's end is to mean the other's too, for which one CTA waits; the rest make room
+  // for CTAs that have not run yet (all waiting: 76.0 instead of 75.3 us for 96 rows behind
+  // 32832 keys, 68 instead of 64 for 8 padded prompts behind 4000).
+  if (a.behind && blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
