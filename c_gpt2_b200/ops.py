@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -452,14 +453,15 @@ def _pools(K: torch.Tensor, V: torch.Tensor, dev: int, names: str):
     shape = K.shape
     if V.shape != shape or len(shape) < 2:
         raise ValueError(f"{names}: expected pools of one shape, pages first")
+    size = math.prod(shape[1:])
     if K.is_contiguous() and V.is_contiguous():
-        size = stride = K.stride(0)
+        stride = size  # (the first dimension's own says nothing where that has one page)
     else:
-        strides, size = K.stride(), 1
+        strides, inner = K.stride(), 1
         for n, s in zip(reversed(shape[1:]), reversed(strides[1:])):
-            if n != 1 and s != size:
+            if n != 1 and s != inner:
                 raise ValueError(f"{names}: expected contiguous pages")
-            size *= n
+            inner *= n
         if V.stride() != strides:
             raise ValueError(f"{names}: expected equally strided pools")
         stride = strides[0] if shape[0] > 1 else size

@@ -122,6 +122,23 @@ def test_page_cache_takes_one_page_and_strided_pages():
     assert _cpu_cache(K=kv[:, 0], V=kv[:, 1]).c.page_stride == 2 * 2 * 3 * 16 * 64
 
 
+@pytest.mark.parametrize("pools", [
+    lambda n: (lambda kv: (kv[n - 1:, 0], kv[n - 1:, 1]))(
+        torch.zeros(n, 2, 3, 4, 16, 64, dtype=torch.bfloat16)),   # a page of K and V side by side
+    lambda n: (lambda k: (k, k.clone().transpose(0, 1).contiguous().transpose(0, 1)))(
+        torch.zeros(3, 1, 4, 16, 64, dtype=torch.bfloat16).transpose(0, 1)),  # layers first
+    lambda n: (lambda k: (k[2:3], k[1:2]))(torch.zeros(n, 3, 4, 16, 64, dtype=torch.bfloat16)),
+    lambda n: (lambda k: (k[::4][-1:], k[1::4][-1:]))(
+        torch.zeros(n, 3, 4, 16, 64, dtype=torch.bfloat16)),      # every fourth page, the last one
+])
+def test_a_pool_of_one_page_has_its_page_size(pools):
+    """The stride of a dimension of length one says nothing of a page's size."""
+    K, V = pools(9)
+    assert K.shape == V.shape == (1, 3, 4, 16, 64)
+    size, stride = ops._pools(K, V, -1, "K, V")[3:]
+    assert size == 3 * 4 * 16 * 64 and stride == size
+
+
 # ---- the oracle itself ------------------------------------------------------
 
 def test_oracle_keeps_its_books():

@@ -197,6 +197,34 @@ def test_copy_between_pools(cuda, shape):
     assert torch.equal(K2, wk) and torch.equal(V2, wv)
 
 
+@pytest.mark.parametrize("which", ["source", "destination", "both", "layers first"])
+def test_copy_of_one_page_pools(cuda, which):
+    """One page out of a pool whose pages hold K and V side by side: its neighbours in
+    both pools, which one page too many would reach, stay as they are."""
+    L, G, page, n = 3, 2, 16, 6
+    g = torch.Generator(device=cuda).manual_seed(3)
+    a = torch.randn(n, 2, L, G, page, 64, generator=g, device=cuda).bfloat16()
+    b = torch.randn(n, 2, L, G, page, 64, generator=g, device=cuda).bfloat16()
+    one_src, one_dst = which in ("source", "both"), which in ("destination", "both")
+    ks, vs = (a[2:3, 0], a[2:3, 1]) if one_src else (a[:, 0], a[:, 1])
+    if which == "layers first":  # one page, [L, 1, ...] transposed
+        a = torch.randn(L, 1, G, page, 64, generator=g, device=cuda).bfloat16()
+        w = torch.randn(L, 1, G, page, 64, generator=g, device=cuda).bfloat16()
+        ks, vs, one_src = a.transpose(0, 1), w.transpose(0, 1), True
+    kd, vd = (b[3:4, 0], b[3:4, 1]) if one_dst else (b[:, 0], b[:, 1])
+    want = b.clone()
+    want[3, 0] = ks[0 if one_src else 2]
+    want[3, 1] = vs[0 if one_src else 2]
+    before = a.clone()
+    ops.pages_copy(ks, vs, i32([0 if one_src else 2]), kd, vd, i32([0 if one_dst else 3]))
+    assert torch.equal(b, want) and torch.equal(a, before)
+    # and the densely packed pool
+    dense = torch.zeros(1, L, G, page, 64, dtype=torch.bfloat16, device=cuda)
+    k2, v2 = dense.clone(), dense.clone()
+    ops.pages_copy(ks, vs, i32([0 if one_src else 2]), k2, v2, i32([0]))
+    assert torch.equal(k2, want[3:4, 0]) and torch.equal(v2, want[3:4, 1])
+
+
 # ---- attention --------------------------------------------------------------
 
 def build(cuda, n_seq, T, H, G, page, n_shared, tails, n_new, seed, n_layer=2, layer=1, scale=1.5,
