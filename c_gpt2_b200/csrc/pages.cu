@@ -488,12 +488,21 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------
-static int book_smem(const void *kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return W8A8_OK;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
-                 cudaSuccess
-             ? W8A8_OK
-             : W8A8_ERR_CUDA;
+// The fork's lists at their longest, allowed once a device and never lowered: a call's own size
+// would be for calls of other threads too, and the default 48 KB hold the kernel's static
+// shared memory as well.
+static int fork_book_opt_in() {
+  static bool done[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return W8A8_ERR_CUDA;
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(pages_fork_book_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             3 * W8A8_PAGES_MAX_LIST * (int)sizeof(int)) != cudaSuccess)
+      return W8A8_ERR_CUDA;
+    done[dev] = true;
+  }
+  return W8A8_OK;
 }
 
 int launch_pages_extend(const PagesArgs &a, const int32_t *n_new, int32_t *pos0, cudaStream_t s) {
@@ -517,7 +526,7 @@ int launch_pages_write(const PagesArgs &a, int layer, const uint16_t *Kn, int64_
 int launch_pages_fork(const PagesArgs &a, const int32_t *src, const int32_t *dst, int n,
                       int32_t *status, int sm_count, cudaStream_t s) {
   const size_t smem = ((size_t)a.n_slot + 2 * (size_t)n) * 4;
-  int st = book_smem((const void *)pages_fork_book_kernel, smem);
+  int st = fork_book_opt_in();
   if (st) return st;
   launch_pdl(pages_fork_book_kernel, dim3(1), dim3(kBookThreads), smem, s, a, src, dst, n, status);
   st = check_launch("pages_fork_book");

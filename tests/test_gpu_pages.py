@@ -127,6 +127,37 @@ def test_fork_runs_out_of_pages_in_list_order(cuda):
     assert b.refs.sum() == 2
 
 
+_FORK_FIRST = """
+import sys
+import torch
+from c_gpt2_b200 import ops
+from c_gpt2_b200.pages import PageCache
+ops.init(0)
+for n_slot, n in (%s):
+    i32 = dict(dtype=torch.int32, device="cuda:0")
+    c = PageCache.empty(n + 1, n_slot, 1, 1, 1, 16, "cuda:0")
+    n_new = torch.zeros(n_slot, **i32)
+    n_new[0] = 5
+    ops.pages_extend(c, n_new)
+    dst = torch.arange(n, **i32)
+    status = ops.pages_fork(c, torch.zeros_like(dst), dst)
+    assert status.tolist() == [1] + [0] * (n - 1), (n_slot, n)
+    assert c.n_ctx[:n].tolist() == [5] * n and c.table[:n, 0].tolist() == list(range(n))
+assert ops.device_error() == 0
+"""
+
+
+def test_a_first_fork_whose_lists_fill_the_default_shared_memory(cuda):
+    """n_slot + 2 n words at 48 KB and just below it, where the kernel's static shared
+    memory comes on top, as the first forks of a process; then smaller ones and the largest."""
+    import subprocess
+    import sys
+    for sizes in ("(4096, 4096), (64, 9), (8192, 8192)", "(8192, 2040), (4096, 4090), (2, 2)"):
+        r = subprocess.run([sys.executable, "-c", _FORK_FIRST % sizes], capture_output=True,
+                           text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_bad_entries_are_skipped_and_recorded(cuda):
     """Table entries outside the pool: nothing is followed, the error word is set."""
     for bad in (-7, 5, 2 ** 31 - 1):
