@@ -211,7 +211,7 @@ struct Item {
   int b, nn;    // sequence of a tail and its new rows; -1: prefix
   int kvh, r0;  // key head; first row of the tile among the (m, g) rows of b or of all
   int k0, k1;   // positions
-  int n_valid;  // positions that hold anything
+  int n_valid;  // positions that hold anything, of a prefix: that some query sees
   int warps;    // where `begins`: warps that share the group
   bool begins, ends;
 };
@@ -236,13 +236,22 @@ __device__ __forceinline__ int row_tiles(const ApArgs &a, int nn) {
   return (nn * a.g + kRows - 1) / kRows;
 }
 
-__device__ __forceinline__ int all_stages(const ApArgs &a, int lane) {
-  int v = 0;
+// All groups' stages; *prefix: the shared positions that some query sees. (Those behind may hold
+// anything: their values are left out of the products, where 0 * NaN would not stay 0.)
+__device__ __forceinline__ int all_stages(const ApArgs &a, int lane, int *prefix) {
+  int v = 0, seen = 0;
 #pragma unroll 4
-  for (int b = lane; b < a.n_seq; b += 32)
-    v += tail_stages(a, seq_len(a, b)) * row_tiles(a, seq_new(a, b));
+  for (int b = lane; b < a.n_seq; b += 32) {
+    const int len = seq_len(a, b), nn = seq_new(a, b);
+    v += tail_stages(a, len) * row_tiles(a, nn);
+    if (nn > 0) seen = max(seen, len);
+  }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  for (int d = 16; d; d >>= 1) {
+    v += __shfl_xor_sync(~0u, v, d);
+    seen = max(seen, __shfl_xor_sync(~0u, seen, d));
+  }
+  *prefix = min(seen, a.n_shared);
   return (a.p_tiles * a.p_stages + v) * a.n_kv;
 }
 
@@ -278,7 +287,7 @@ __device__ __forceinline__ void walk_next_seq(const ApArgs &a, Walk &w, int lane
 }
 
 __device__ __forceinline__ Walk walk_begin(const ApArgs &a, int me, int per_warp, int all,
-                                           int lane) {
+                                           int prefix, int lane) {
   Walk w = {};
   w.me = me;
   w.per_warp = per_warp;
@@ -291,7 +300,7 @@ __device__ __forceinline__ Walk walk_begin(const ApArgs &a, int me, int per_warp
     w.b = -1;
     w.st = a.p_stages;
     w.tiles = a.p_tiles;
-    w.n_valid = a.n_shared;
+    w.n_valid = prefix;
   } else {
     x -= pre;
     int l;
@@ -336,7 +345,7 @@ __device__ __forceinline__ Item walk_next(const ApArgs &a, Walk &w, int lane) {
   it.k0 = w.s0 * kStageKeys;
   it.k1 = it.k0 + n * kStageKeys;
   if (it.b < 0) {
-    it.k1 = min(it.k1, a.n_shared);
+    it.k1 = min(it.k1, it.n_valid);
   } else {
     it.k0 += a.base;
     // the last row of the tile sees furthest
@@ -515,10 +524,11 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
 
   // neighbouring stretches on different SMs: they share keys in L2, and few stages spread out
   const int me = warp * gridDim.x + blockIdx.x;
-  const int all = all_stages(a, lane), unit = max(a.whole, 1);
+  int prefix;
+  const int all = all_stages(a, lane, &prefix), unit = max(a.whole, 1);
   const int warps = gridDim.x * kMmaWarps;
   const int per_warp = max((all / unit + warps - 1) / warps, 1) * unit;
-  Walk walk = walk_begin(a, me, per_warp, all, lane);
+  Walk walk = walk_begin(a, me, per_warp, all, prefix, lane);
 
   // ---- loading: lane i < 2 * boxes brings one box (16 to 64 rows) of a stage ----
   const int box = min(1 << a.page_shift, kStageKeys);
@@ -733,13 +743,22 @@ struct TcItem {
 };
 
 // The items over the prefix; how many rows of a padded batch hold a query is known here only.
-__device__ __forceinline__ Across plan_across(const ApArgs &a, int lane) {
-  if (!a.n_new) return a.across;
-  int valid = 0;
+// *prefix: the shared positions that some query sees (see all_stages).
+__device__ __forceinline__ Across plan_across(const ApArgs &a, int lane, int *prefix) {
+  int valid = 0, seen = 0;
 #pragma unroll 4
-  for (int b = lane; b < a.n_seq; b += 32) valid += seq_new(a, b);
+  for (int b = lane; b < a.n_seq; b += 32) {
+    const int nn = seq_new(a, b), len = seq_len(a, b);
+    valid += nn;
+    if (nn > 0) seen = max(seen, len);
+  }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) valid += __shfl_xor_sync(~0u, valid, d);
+  for (int d = 16; d; d >>= 1) {
+    valid += __shfl_xor_sync(~0u, valid, d);
+    seen = max(seen, __shfl_xor_sync(~0u, seen, d));
+  }
+  *prefix = min(seen, a.n_shared);
+  if (!a.n_new) return a.across;
   Across p = across_of(valid * a.g, a.n_kv, a.n_shared, lane + 1, a.tc);
   int best = p.cost << 5 | lane;  // a lane a choice
 #pragma unroll
@@ -772,23 +791,24 @@ __device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx, int lane
     it.k1 = min(it.k0 + a.chunk, end);
     return it;
   }
-  const Across p = plan_across(a, lane);
+  int prefix;
+  const Across p = plan_across(a, lane, &prefix);
   const int full = p.pairs * p.s2, each = full + p.s1;
   it.b = -1;
   it.kvh = each ? idx / each : a.n_kv;
   it.r0 = it.r1 = it.k0 = it.k1 = it.splits = 0;
-  it.n_valid = a.n_shared;
+  it.n_valid = prefix;
   if (it.kvh >= a.n_kv) return it;  // one CTA too many
   const int q = idx - it.kvh * each;
   const bool one = q >= full;
   const int pair = one ? p.pairs : q / p.s2;
   const int chunk = one ? p.c1 : p.c2;
   it.split = one ? q - full : q - pair * p.s2;
-  it.splits = one ? p.s1 : p.s2;
+  it.splits = (prefix + chunk - 1) / chunk;  // with keys; the others leave no part
   it.r0 = pair * kPairRows;
   it.r1 = min(it.r0 + kPairRows, p.rows);
   it.k0 = it.split * chunk;
-  it.k1 = min(it.k0 + chunk, a.n_shared);
+  it.k1 = min(it.k0 + chunk, prefix);
   return it;
 }
 

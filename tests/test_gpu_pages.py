@@ -402,6 +402,70 @@ def test_keys_nobody_sees_may_hold_anything(cuda, n_seq, T):
         assert torch.equal(outs[0].view(torch.int16), o.view(torch.int16))
 
 
+# the plans: whole 16-row groups, a prefix shared out to 16-row groups, tensor-core items over
+# the prefix (two and, of few rows, one tile wide), and over a sequence's whole keys
+PLANS = [
+    # n_seq, T, H, G, page, n_shared, longest tail
+    (3, 2, 4, 2, 16, 64, 40),
+    (3, 2, 4, 2, 32, 320, 100),
+    (150, 2, 8, 8, 64, 1728, 30),
+    (60, 2, 16, 16, 16, 2304, 30),
+    (2, 70, 4, 2, 32, 64, 2300),
+    (2, 90, 4, 2, 64, 192, 100),
+]
+
+
+def sees(c, Q, T, H, lens, n_new, layer=1):
+    """(O, A) of the 64-bit oracle where sequence b holds lens[b] positions, n_new[b] of them
+    new, of which the first T at most have a row."""
+    G, n_seq = c.n_kv_head, len(lens)
+    k64, v64 = (t[:, layer].double().cpu().numpy() for t in (c.K, c.V))
+    table = c.table.cpu().numpy()
+    q64 = Q.double().cpu().numpy().reshape(n_seq, T, H, 64)
+    want = []
+    for b, (n, new) in enumerate(zip(lens, n_new)):
+        n = max(n - max(new - T, 0), 0)  # what the last row sees
+        p = table[b, :-(-n // c.page)]
+        kb, vb = (x[p].transpose(0, 2, 1, 3).reshape(-1, G, 64)[:n] for x in (k64, v64))
+        want.append(po.attention(q64[b], kb, vb, min(new, T)))
+    return want
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("inside", ["page", "block", "idle", "nothing"])
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_prefix_that_nobody_sees_the_end_of(cuda, plan, inside, padded):
+    """Every sequence with a query ends inside the shared pages: what stands behind the
+    longest of them, there too, may hold anything."""
+    n_seq, T, H, G, page, n_shared, tail = plan
+    c, Q, shared, _ = build(cuda, n_seq, T, H, G, page, n_shared, [tail] * n_seq, [T] * n_seq, 4)
+    longest = {"page": n_shared - 3, "block": n_shared // 2 + 5, "idle": n_shared // 3,
+               "nothing": 0}[inside]
+    lens = [max(longest - 2 * b, 0) for b in range(n_seq)]
+    n_new = [T] * n_seq
+    if padded:
+        n_new = [T - b % 2 for b in range(n_seq)]
+    if inside == "idle":  # one that reaches the end, without a query
+        if not padded:
+            pytest.skip("n_new None: every sequence has queries")
+        lens[-1], n_new[-1] = n_shared + tail, 0
+    c.n_ctx.copy_(i32(lens))
+    seen = torch.zeros(c.n_pages, page, dtype=torch.bool, device=cuda)
+    flat = shared.long()[:, None] * page + torch.arange(page, device=cuda)
+    seen.view(-1)[flat.view(-1)[:longest]] = True
+    outs = []
+    for junk in (0.0, float("nan"), float("inf")):
+        for pool in (c.K, c.V):
+            pool.permute(0, 3, 1, 2, 4)[~seen] = junk
+        out = torch.full((n_seq * T, H * 64), 7.0, dtype=torch.bfloat16, device=cuda)
+        ops.attention_pages(Q, c, 1, H, T=T, n_new=i32(n_new) if padded else None,
+                            max_ctx=n_shared + tail, shared_pages=shared, n_shared=n_shared, out=out)
+        if junk == 0.0:
+            check(out, sees(c, Q, T, H, lens, n_new), T, H, n_new)
+        outs.append(out.view(torch.int16))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 @pytest.mark.parametrize("T,n_shared", [(3, 0), (3, 320), (70, 32), (300, 0)])
 def test_a_key_that_is_not_a_number(cuda, T, n_shared):
     """NaN in the newest position's key reaches the row that sees it and no other."""
