@@ -237,7 +237,7 @@ __device__ __forceinline__ int row_tiles(const ApArgs &a, int nn) {
 }
 
 // All groups' stages; *prefix: the shared positions that some query sees. (Those behind may hold
-// anything: their values are left out of the products, where 0 * NaN would not stay 0.)
+// anything: their values are kept out of the products, where 0 * NaN would not stay 0.)
 __device__ __forceinline__ int all_stages(const ApArgs &a, int lane, int *prefix) {
   int v = 0, seen = 0;
 #pragma unroll 4
@@ -246,13 +246,8 @@ __device__ __forceinline__ int all_stages(const ApArgs &a, int lane, int *prefix
     v += tail_stages(a, len) * row_tiles(a, nn);
     if (nn > 0) seen = max(seen, len);
   }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    v += __shfl_xor_sync(~0u, v, d);
-    seen = max(seen, __shfl_xor_sync(~0u, seen, d));
-  }
-  *prefix = min(seen, a.n_shared);
-  return (a.p_tiles * a.p_stages + v) * a.n_kv;
+  *prefix = min(__reduce_max_sync(~0u, seen), a.n_shared);
+  return (a.p_tiles * a.p_stages + __reduce_add_sync(~0u, v)) * a.n_kv;
 }
 
 // The next 32 sequences; returns this lane's stages.
@@ -731,6 +726,7 @@ struct TcCtl {
   uint64_t v_ready, drain;
   uint32_t tmem_base;
   int abort_flag;
+  int cut;  // the block inside which the positions end that some query sees, -1: none
   int idle[8];
   float2 ml[kTileRows];  // group 1's, where both groups work on one tile
 };
@@ -743,22 +739,12 @@ struct TcItem {
 };
 
 // The items over the prefix; how many rows of a padded batch hold a query is known here only.
-// *prefix: the shared positions that some query sees (see all_stages).
-__device__ __forceinline__ Across plan_across(const ApArgs &a, int lane, int *prefix) {
-  int valid = 0, seen = 0;
-#pragma unroll 4
-  for (int b = lane; b < a.n_seq; b += 32) {
-    const int nn = seq_new(a, b), len = seq_len(a, b);
-    valid += nn;
-    if (nn > 0) seen = max(seen, len);
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    valid += __shfl_xor_sync(~0u, valid, d);
-    seen = max(seen, __shfl_xor_sync(~0u, seen, d));
-  }
-  *prefix = min(seen, a.n_shared);
+__device__ __forceinline__ Across plan_across(const ApArgs &a, int lane) {
   if (!a.n_new) return a.across;
+  int valid = 0;
+#pragma unroll 4
+  for (int b = lane; b < a.n_seq; b += 32) valid += seq_new(a, b);
+  valid = __reduce_add_sync(~0u, valid);
   Across p = across_of(valid * a.g, a.n_kv, a.n_shared, lane + 1, a.tc);
   int best = p.cost << 5 | lane;  // a lane a choice
 #pragma unroll
@@ -791,24 +777,23 @@ __device__ __forceinline__ TcItem get_tc_item(const ApArgs &a, int idx, int lane
     it.k1 = min(it.k0 + a.chunk, end);
     return it;
   }
-  int prefix;
-  const Across p = plan_across(a, lane, &prefix);
+  const Across p = plan_across(a, lane);
   const int full = p.pairs * p.s2, each = full + p.s1;
   it.b = -1;
   it.kvh = each ? idx / each : a.n_kv;
   it.r0 = it.r1 = it.k0 = it.k1 = it.splits = 0;
-  it.n_valid = prefix;
+  it.n_valid = a.n_shared;
   if (it.kvh >= a.n_kv) return it;  // one CTA too many
   const int q = idx - it.kvh * each;
   const bool one = q >= full;
   const int pair = one ? p.pairs : q / p.s2;
   const int chunk = one ? p.c1 : p.c2;
   it.split = one ? q - full : q - pair * p.s2;
-  it.splits = (prefix + chunk - 1) / chunk;  // with keys; the others leave no part
+  it.splits = one ? p.s1 : p.s2;
   it.r0 = pair * kPairRows;
   it.r1 = min(it.r0 + kPairRows, p.rows);
   it.k0 = it.split * chunk;
-  it.k1 = min(it.k0 + chunk, prefix);
+  it.k1 = min(it.k0 + chunk, a.n_shared);
   return it;
 }
 
@@ -889,8 +874,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // an item without keys leaves no part, unless rows get their zeros here
   if (blocks == 0 && !a.direct && it.split > 0) return;
   const int units = one ? blocks : 2 * blocks;  // unit u: group u & 1
-  // the last block reaches behind the positions that hold anything
-  const bool v_cut = it.k0 + blocks * kTcKeys > it.n_valid;
   if (threadIdx.x == 0) {
     mbar_init(&ctl->q_full, 8);
     for (int i = 0; i < kTcStages; ++i) {
@@ -1165,24 +1148,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool act = lane < 2 * boxes;
     const bool is_v = lane >= boxes;
     const int bx = is_v ? lane - boxes : lane;
-    auto entry = [&](int j) -> int {  // page of this lane's box, n_pages: reads as zeros
-      const int pos = it.k0 + j * kTcKeys + bx * box;
-      if (!act || pos >= it.k1) return a.n_pages;
-      const int k = pos >> a.page_shift;
-      int p = -1;
-      if (pos < a.n_shared) p = a.shared[k];
-      else if (k < a.max_pages) p = a.table[(int64_t)it.b * a.max_pages + k];
-      if (p < 0 || p >= a.n_pages) {
+    // page of this lane's box of a block, as the lists have it (any value behind the item's keys)
+    auto fetch = [&](int j) -> int {
+      const int pos = it.k0 + j * kTcKeys + bx * box, k = pos >> a.page_shift;
+      if (!act || pos >= it.k1) return -1;
+      if (pos < a.n_shared) return a.shared[k];
+      return k < a.max_pages ? a.table[(int64_t)it.b * a.max_pages + k] : -1;
+    };
+    int p = blocks ? fetch(0) : 0;
+    // Positions that some query sees (see all_stages), counted while the first entries arrive;
+    // no other warp waits for it (all of them: 75 -> 77 us for 96 rows behind 32832 keys). Boxes
+    // behind read as zeros, and the rest of a block inside which they end is overwritten.
+    int valid = it.n_valid;
+    if (it.b < 0) {
+      int seen = 0;
+#pragma unroll 4
+      for (int b = lane; b < a.n_seq; b += 32)
+        if (seq_new(a, b) > 0) seen = max(seen, seq_len(a, b));
+      valid = min(__reduce_max_sync(~0u, seen), a.n_shared);
+    }
+    const int k1 = min(it.k1, valid), rest = valid - it.k0;
+    const int cut = rest > 0 && rest < blocks * kTcKeys && rest % kTcKeys ? rest / kTcKeys : -1;
+    if (lane == 0) ctl->cut = cut;  // (released by the first arrival below)
+    int n = 0;
+    for (; n < blocks; ++n) {
+      const int next = n + 1 < blocks ? fetch(n + 1) : 0;
+      const int st = n % kTcStages;
+      const int pos = it.k0 + n * kTcKeys + bx * box;
+      if (!act || pos >= k1) {
+        p = a.n_pages;  // reads as zeros
+      } else if (p < 0 || p >= a.n_pages) {
         report_error(a.err, kErrEntry);
         p = a.n_pages;
       }
-      return p;
-    };
-    int p = blocks ? entry(0) : 0;
-    int n = 0;
-    for (; n < blocks; ++n) {
-      const int next = n + 1 < blocks ? entry(n + 1) : 0;
-      const int st = n % kTcStages;
       bool ok = true;
       if (n >= kTcStages)
         ok = mbar_wait(&ctl->kv_empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag, a.err, kErrTc);
@@ -1190,19 +1188,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive_expect_tx(&ctl->kv_full[st], 2 * kTcTile);
       __syncwarp();
       if (act) {
-        const int pos = it.k0 + n * kTcKeys + bx * box;
         const int y = (it.kvh << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
         tma_load_3d(sKV + (st * 2 + is_v) * kTcTile + bx * box * 128, is_v ? &tmV : &tmK,
                     &ctl->kv_full[st], 0, y, p);
       }
       p = next;
-    }
-    if (n == blocks && v_cut) {
-      // rows of the last page that hold nothing yet: 0 * V must stay 0
-      const int j = blocks - 1, st = j % kTcStages;
-      if (mbar_wait(&ctl->kv_full[st], (j / kTcStages) & 1, abort_flag, a.err, kErrTc + 1)) {
+      if (n == cut && __all_sync(~0u, mbar_wait(&ctl->kv_full[st], (n / kTcStages) & 1, abort_flag,
+                                                a.err, kErrTc + 1))) {
         uint8_t *v = sKV + (st * 2 + 1) * kTcTile;
-        for (int x = (it.n_valid - it.k0 - j * kTcKeys) * 8 + lane; x < kTcKeys * 8; x += 32)
+        for (int x = rest % kTcKeys * 8 + lane; x < kTcKeys * 8; x += 32)
           *reinterpret_cast<uint4 *>(v + x * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
@@ -1225,6 +1219,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int mine = (units - g + 1) / 2;
       bool ok = mine > 0 && mbar_wait(&ctl->q_full, 0, abort_flag, a.err, kErrTc + 2);
       int seen = 0;  // blocks that have been in shared memory
+      int cut = -1;
       auto issue_s = [&](int i) -> bool {
         const int j = one ? 2 * i + g : i;  // block
         if (i > 0 && !mbar_wait(&ctl->s_free[g], (i - 1) & 1, abort_flag, a.err, kErrTc + 3))
@@ -1245,9 +1240,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       auto issue_o = [&](int i) -> bool {
         const int j = one ? 2 * i + g : i;
         if (!mbar_wait(&ctl->p_full[g], i & 1, abort_flag, a.err, kErrTc + 5)) return false;
-        if (v_cut && j == blocks - 1 &&
-            !mbar_wait(&ctl->v_ready, 0, abort_flag, a.err, kErrTc + 10))
-          return false;
+        if (j == cut && !mbar_wait(&ctl->v_ready, 0, abort_flag, a.err, kErrTc + 10)) return false;
         tc_fence_after();
         tc_mma_bf16_ta_x8(base + kColO, base + kColP, v_desc + (j % kTcStages) * (2 * kTcTile >> 4),
                           idO, i > 0);
@@ -1256,6 +1249,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return true;
       };
       if (ok) ok = issue_s(0);
+      if (ok) cut = *(volatile int *)&ctl->cut;  // written before the first block's arrival
       for (int i = 0; i < mine && ok; ++i) {
         if (i + 1 < mine) ok = issue_s(i + 1);
         if (ok) ok = issue_o(i);
