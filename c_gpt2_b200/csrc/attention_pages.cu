@@ -130,8 +130,11 @@ struct ApArgs {
   int *err;
 };
 
+// Positions up to the one that the last row sees: where more are new than there are rows, the
+// rows are the first of them.
 __device__ __forceinline__ int seq_len(const ApArgs &a, int b) {
-  return min(max(a.n_ctx[b], 0), a.max_ctx);
+  const int len = min(max(a.n_ctx[b], 0), a.max_ctx);
+  return a.n_new ? max(len - max(a.n_new[b] - a.T, 0), 0) : len;
 }
 __device__ __forceinline__ int seq_new(const ApArgs &a, int b) {
   return a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;

@@ -338,9 +338,10 @@ int w8a8_pages_copy(const gpt2_bf16_t *Ksrc, const gpt2_bf16_t *Vsrc, int64_t sr
 /* ---- attention over the pages, a shared prefix read once ----
  * T query rows a sequence, a padded batch: row m = b*T + t, head h reads
  * Q[m*ldq + h*64 ..], for b < n_seq <= n_slot and t < n_new[b] (device, NULL:
- * all T); slot b's n_ctx[b] positions include the new ones. Row t attends the
- * positions below end = min(n_ctx[b], max_ctx) - n_new[b] + t + 1 of key head
- * h / (n_head / n_kv_head):
+ * all T); slot b's n_ctx[b] positions include the n_new[b] new ones, of which the
+ * rows are the first, as in w8a8_pages_write (n_new[b] may exceed T). Row t
+ * attends the positions below end = min(n_ctx[b], max_ctx) - n_new[b] + t + 1 of
+ * key head h / (n_head / n_kv_head):
  *   O[m*ldo + h*64 ..] = bf16(softmax_j(q.k_j / 8) . V),  fp32 scores, maxima,
  *   sums and accumulators; the weights are rounded to bf16 for the product with V.
  * A row with end <= 0 is written as zeros; rows t >= n_new[b] are left as they

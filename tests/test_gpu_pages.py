@@ -466,6 +466,44 @@ def test_a_prefix_that_nobody_sees_the_end_of(cuda, plan, inside, padded):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("plan", PLANS)
+def test_more_new_positions_than_rows(cuda, plan):
+    """n_new[b] > T: the T rows are the first of the new positions, as pages_write places
+    them, and what follows them may hold anything."""
+    n_seq, T, H, G, page, n_shared, tail = plan
+    tails = [tail - b % 9 for b in range(n_seq)]
+    n_new = [(T, T + 1, T + 7, T - 1, T + 2 * page)[b % 5] for b in range(n_seq)]
+    n_new[0] = T + 3
+    lens = [n_shared + t for t in tails]
+    lens[-1], n_new[-1] = n_shared + 1, T + n_shared  # rows before any position, the last at one
+    c, Q, shared, _ = build(cuda, n_seq, T, H, G, page, n_shared, tails, [T] * n_seq, 6)
+    c.n_ctx.copy_(i32(lens))
+    for b in range(n_seq):  # positions of its own behind the last row
+        for pos in range(max(lens[b] - max(n_new[b] - T, 0), n_shared), n_shared + tails[b]):
+            for pool in (c.K, c.V):
+                pool[c.table[b, pos // page].long(), :, :, pos % page] = float("nan")
+    out = torch.full((n_seq * T, H * 64), 7.0, dtype=torch.bfloat16, device=cuda)
+    ops.attention_pages(Q, c, 1, H, T=T, n_new=i32(n_new), max_ctx=n_shared + tail,
+                        shared_pages=shared, n_shared=n_shared, out=out)
+    check(out, sees(c, Q, T, H, lens, n_new), T, H, [min(n, T) for n in n_new])
+    # lengths and counts at the ends of 32 bits
+    c.n_ctx[0], c.n_ctx[1] = -2 ** 31, lens[1]
+    far = i32([2 ** 31 - 1, -2 ** 31] + n_new[2:])
+    out.fill_(7.0)
+    ops.attention_pages(Q, c, 1, H, T=T, n_new=far, max_ctx=n_shared + tail, shared_pages=shared,
+                        n_shared=n_shared, out=out)
+    check(out, sees(c, Q, T, H, [0, 0] + lens[2:], [T, 0] + n_new[2:]), T, H,
+          [T, 0] + [min(n, T) for n in n_new[2:]])
+    c.n_ctx[0] = lens[0]
+    # a bound below the lengths cuts them first
+    cut = n_shared + tail // 2
+    out.fill_(7.0)
+    ops.attention_pages(Q, c, 1, H, T=T, n_new=i32(n_new), max_ctx=cut, shared_pages=shared,
+                        n_shared=n_shared, out=out)
+    want = sees(c, Q, T, H, [min(n, cut) for n in lens], n_new)
+    check(out, want, T, H, [min(n, T) for n in n_new])
+
+
 @pytest.mark.parametrize("T,n_shared", [(3, 0), (3, 320), (70, 32), (300, 0)])
 def test_a_key_that_is_not_a_number(cuda, T, n_shared):
     """NaN in the newest position's key reaches the row that sees it and no other."""
