@@ -622,6 +622,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
       }
     w.m[0] = w.m[1] = -INFINITY;
     w.l[0] = w.l[1] = 0.0f;
+    bool late = false;  // a copy that did not arrive: the warp has no more to do, but ends below
     for (int s = 0; s < stages; ++s, ++n) {
       load();  // into the stage that was read last
       const int st = n % kStages;
@@ -629,7 +630,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
         // no copy may still be writing shared memory when the warp exits
         for (uint32_t i = n + 1; i < loaded; ++i)
           mbar_wait(&full[i % kStages], (i / kStages) & 1, nullptr, a.err, kErrWaitFull);
-        return;
+        late = true;
+        break;
       }
       const int key0 = it.k0 + s * kStageKeys;
       uint8_t *sK = ring + st * 2 * kTileBytes, *sV = sK + kTileBytes;
@@ -645,6 +647,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
       else mma_stage<false>(w, smem_u32(sK), smem_u32(sV), lim, lane);
       __syncwarp();  // reads of this stage, then the copy that the next load() starts into it
     }
+    if (late) break;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       float l = w.l[r];
