@@ -205,6 +205,12 @@ __device__ __forceinline__ bool grown(float top, float m) {
   return top > m && !((top - m) * kScale2 <= kMaxSlack);
 }
 
+// A load after which nothing is read from L1 that was there before it.
+__device__ __forceinline__ void load_acquire(const int *p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+}
+
 struct MmaSmem {
   uint64_t full[kMmaWarps][kStages];
 };
@@ -514,11 +520,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 1)
     }
   }
   __syncwarp();
-  // Behind the tensor-core kernel, which lets this one start once all its CTAs run (and what
-  // came before it is complete), there is nothing to wait for before the end: both only write
-  // parts of rows, and a CTA here starts as an SM is free.
+  // Behind the tensor-core kernel there is nothing to wait for before the end: both only write
+  // parts of rows, and a CTA here starts as an SM is free. What came before that kernel is
+  // complete, with its writes in memory: each of its CTAs waited for that before it let this
+  // kernel start. TMA reads from there; for the plain loads, the acquire drops what this SM's L1
+  // may hold of older contents (0.1 us a call; a full fence 1.2).
   pdl_launch_dependents();
-  if (!a.behind) pdl_wait();
+  if (a.behind) load_acquire(a.n_ctx);
+  else pdl_wait();
 
   // neighbouring stretches on different SMs: they share keys in L2, and few stages spread out
   const int me = warp * gridDim.x + blockIdx.x;

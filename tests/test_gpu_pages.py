@@ -650,6 +650,56 @@ def test_another_stream_and_captured_graphs(cuda):
     assert ca.refs.sum().item() == 4 * 5 and ca.table[:, :2].unique().numel() == 2
 
 
+def test_captured_steps_behind_a_long_prefix(cuda):
+    """A captured step whose 16-row kernel runs behind the tensor-core kernel: lengths,
+    table, rows and queries of each replay are the ones that it reads, as in eager steps
+    into a cache of their own, with a wait after every call."""
+    n_seq, G, H, page, ns = 100, 16, 16, 16, 144
+    src, _ = make(cuda, ns + 5 * n_seq, n_seq, ns + 5, n_layer=1, n_kv=G, page=page, seed=2)
+    shared = torch.arange(ns, device=cuda, dtype=torch.int32)
+    src.table[:, :ns] = shared
+    src.n_ctx.fill_(ns * page)
+    src.refs[:ns] = n_seq
+    caches = [PageCache(*(t.clone() for t in (src.K, src.V, src.table, src.n_ctx, src.refs)))
+              for _ in range(2)]
+    n_new, q = i32([1] * n_seq), torch.zeros(n_seq, H * 64, dtype=torch.bfloat16, device=cuda)
+    x = torch.zeros(n_seq, G * 64, dtype=torch.bfloat16, device=cuda)
+    outs = [torch.zeros_like(q) for _ in range(2)]
+
+    def step(i, wait):
+        c = caches[i]
+        pos0 = ops.pages_extend(c, n_new)
+        wait()
+        ops.pages_write(c, 0, x, x, pos0)
+        wait()
+        ops.attention_pages(q, c, 0, H, n_new=n_new, max_ctx=(ns + 5) * page, shared_pages=shared,
+                            n_shared=ns * page, out=outs[i])
+        wait()
+
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    before = [t.clone() for t in (src.table, src.n_ctx, src.refs)]
+    with torch.cuda.graph(graph, stream=s):
+        for _ in range(3):
+            step(0, lambda: None)
+    g = torch.Generator(device=cuda).manual_seed(8)
+    for t, b in zip((caches[0].table, caches[0].n_ctx, caches[0].refs), before):
+        assert torch.equal(t, b)
+    for i in range(16):
+        x.copy_(torch.randn(x.shape, generator=g, device=cuda))
+        q.copy_(torch.randn(q.shape, generator=g, device=cuda))
+        n_new.copy_((torch.rand(n_seq, generator=g, device=cuda) < 0.7).int())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            step(1, torch.cuda.synchronize)
+        assert torch.equal(outs[0], outs[1]), i
+    for a, b in zip((caches[0].table, caches[0].n_ctx, caches[0].refs),
+                    (caches[1].table, caches[1].n_ctx, caches[1].refs)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("T,n_shared", [(1, 64), (1, 0), (3, 320), (90, 32)])
 def test_strided_rows_and_fewer_sequences_than_slots(cuda, T, n_shared):
     """Q in a packed [Q | K | V] row, an output with padded rows, and the first three
