@@ -544,8 +544,8 @@ extern "C" int w8a8_attention_decode_quant(const gpt2_bf16_t *Q, int64_t ldq,
                                head_dim, O, ldo, Xq, sX, workspace, workspace_bytes, stream);
 }
 
-// Checks a page cache's description; the kernels' form of it in *a.
-static int pages_args(const w8a8_pages *c, PagesArgs *a) {
+// Checks a page cache's description.
+static int pages_check(const w8a8_pages *c) {
   if (!c || !c->K || !c->V || !c->table || !c->n_ctx || !c->refs) return W8A8_ERR_INVALID;
   if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
     return W8A8_ERR_UNSUPPORTED;
@@ -559,7 +559,13 @@ static int pages_args(const w8a8_pages *c, PagesArgs *a) {
   if (c->page_stride < segs * c->page * kPageHd || c->page_stride % 8 || !aligned16(c->K) ||
       !aligned16(c->V))
     return W8A8_ERR_INVALID;
-  int st;
+  return W8A8_OK;
+}
+
+// The kernels' form of a description, once checked, in *a.
+static int pages_args(const w8a8_pages *c, PagesArgs *a) {
+  int st = pages_check(c);
+  if (st) return st;
   DeviceCtx *ctx = device_ctx(&st);
   if (!ctx) return st;
   a->K = c->K;
@@ -671,8 +677,11 @@ static bool attention_pages_sizes(int n_seq, int T, int n_head, int n_kv_head, i
 
 extern "C" size_t w8a8_attention_pages_workspace_size(int n_seq, int T, int n_head, int n_kv_head,
                                                       int max_ctx, int n_shared) {
-  if (!attention_pages_sizes(n_seq, T, n_head, n_kv_head, max_ctx, n_shared)) return 0;
-  return attention_pages_workspace_bytes(n_seq, T, n_head, n_kv_head, max_ctx, n_shared);
+  size_t bytes;
+  if (!attention_pages_sizes(n_seq, T, n_head, n_kv_head, max_ctx, n_shared) ||
+      attention_pages_workspace(n_seq, T, n_head, n_kv_head, max_ctx, n_shared, &bytes))
+    return 0;
+  return bytes;
 }
 
 extern "C" int w8a8_attention_pages(const w8a8_pages *c, int layer, const gpt2_bf16_t *Q,
@@ -680,21 +689,24 @@ extern "C" int w8a8_attention_pages(const w8a8_pages *c, int layer, const gpt2_b
                                     int max_ctx, const int32_t *shared_pages, int n_shared,
                                     int n_head, int head_dim, gpt2_bf16_t *O, int64_t ldo,
                                     void *workspace, size_t workspace_bytes, void *stream) {
-  PagesArgs a;
-  int st = pages_args(c, &a);
+  int st = pages_check(c);
   if (st) return st;
   if (n_seq == 0 || T == 0) return W8A8_OK;
   if (head_dim != kPageHd) return W8A8_ERR_UNSUPPORTED;
-  if (!Q || !O || !workspace || layer < 0 || layer >= a.n_layer || n_seq > a.n_slot ||
-      !attention_pages_sizes(n_seq, T, n_head, a.n_kv_head, max_ctx, n_shared) ||
-      n_shared % a.page || (n_shared > 0 && !shared_pages))
+  if (!Q || !O || layer < 0 || layer >= c->n_layer || n_seq > c->n_slot ||
+      !attention_pages_sizes(n_seq, T, n_head, c->n_kv_head, max_ctx, n_shared) ||
+      n_shared % c->page || (n_shared > 0 && !shared_pages))
     return W8A8_ERR_INVALID;
   const int64_t d = (int64_t)n_head * kPageHd;
-  if (ldq < d || ldo < d || ldq % 8 || ldo % 2 || !aligned16(Q) || ((uintptr_t)O & 3) ||
-      !aligned16(workspace) ||
-      workspace_bytes < attention_pages_workspace_bytes(n_seq, T, n_head, a.n_kv_head, max_ctx,
-                                                        n_shared))
+  if (ldq < d || ldo < d || ldq % 8 || ldo % 2 || !aligned16(Q) || ((uintptr_t)O & 3))
     return W8A8_ERR_INVALID;
+  size_t bytes;  // (calls that are too large have no workspace to look at)
+  st = attention_pages_workspace(n_seq, T, n_head, c->n_kv_head, max_ctx, n_shared, &bytes);
+  if (st) return st;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < bytes) return W8A8_ERR_INVALID;
+  PagesArgs a;
+  st = pages_args(c, &a);
+  if (st) return st;
   AttnPagesCall q = {};
   q.Q = Q;
   q.ldq = ldq;

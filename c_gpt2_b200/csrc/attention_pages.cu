@@ -1475,13 +1475,15 @@ int opt_in_smem(K *kernel, size_t bytes, bool (&done)[64]) {
 }  // namespace
 
 // Parts of rows (64 sums, a maximum and a sum of weights each), and three words a row.
-size_t attention_pages_workspace_bytes(int n_seq, int T, int n_head, int n_kv, int max_ctx,
-                                       int n_shared) {
+int attention_pages_workspace(int n_seq, int T, int n_head, int n_kv, int max_ctx, int n_shared,
+                              size_t *bytes) {
   Plan p;
-  if (make_plan(n_seq, T, n_head, n_kv, max_ctx, n_shared, &p)) return 0;
-  if (p.direct) return 16;
-  return (size_t)p.parts * (kPageHd * sizeof(float) + sizeof(float2)) +
-         3 * sizeof(int) * (size_t)n_seq * T * n_head;
+  const int st = make_plan(n_seq, T, n_head, n_kv, max_ctx, n_shared, &p);
+  if (st) return st;
+  *bytes = p.direct ? 16
+                    : (size_t)p.parts * (kPageHd * sizeof(float) + sizeof(float2)) +
+                          3 * sizeof(int) * (size_t)n_seq * T * n_head;
+  return W8A8_OK;
 }
 
 int launch_attention_pages(const PagesArgs &c, const AttnPagesCall &q, cudaStream_t s) {

@@ -240,8 +240,9 @@ struct AttnPagesCall {
   void *ws;
   size_t ws_bytes;
 };
-size_t attention_pages_workspace_bytes(int n_seq, int T, int n_head, int n_kv_head, int max_ctx,
-                                       int n_shared);
+// W8A8_ERR_UNSUPPORTED where the sizes make more work items than the kernels count.
+int attention_pages_workspace(int n_seq, int T, int n_head, int n_kv_head, int max_ctx,
+                              int n_shared, size_t *bytes);
 int launch_attention_pages(const PagesArgs &a, const AttnPagesCall &c, cudaStream_t s);
 
 }  // namespace w8a8

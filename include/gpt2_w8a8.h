@@ -355,8 +355,9 @@ int w8a8_pages_copy(const gpt2_bf16_t *Ksrc, const gpt2_bf16_t *Vsrc, int64_t sr
  * that share one must not overlap on the GPU) is sized with
  * w8a8_attention_pages_workspace_size, 0 for sizes that are refused; 16-byte
  * aligned Q and workspace, ldq % 8 == 0, O 4-byte aligned, ldo even;
- * n_head % n_kv_head == 0, head_dim 64, n_seq*T*n_head <= 2^30. Calls of more
- * than 2^31 (16 rows x 64 keys) pieces are W8A8_ERR_UNSUPPORTED. The outcome does
+ * n_head % n_kv_head == 0, head_dim 64, n_seq*T*n_head <= 2^30. Calls of some
+ * 2^31 pieces of 16 rows x 64 keys or, where the kernels take 256 rows of one
+ * sequence at a time, of 2^23 such items are W8A8_ERR_UNSUPPORTED. The outcome does
  * not depend on the order in which anything runs. */
 size_t w8a8_attention_pages_workspace_size(int n_seq, int T, int n_head, int n_kv_head,
                                            int max_ctx, int n_shared);

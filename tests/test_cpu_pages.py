@@ -74,6 +74,35 @@ def test_workspace_sizes():
         assert size(*bad) == 0
 
 
+@pytest.mark.parametrize("n_seq,T,n_head,n_kv,max_ctx,n_shared", [
+    (64, 1, 3, 3, 1 << 30, 0),            # 16-row pieces of the sequences' keys
+    (256, 1, 15, 3, 1 << 30, 1 << 29),    # of what follows a prefix
+    (8192, 33, 1100, 1100, 2000, 0),      # items of one sequence's rows
+])
+def test_calls_of_too_many_pieces_are_unsupported(n_seq, T, n_head, n_kv, max_ctx, n_shared):
+    """Said before the workspace is looked at, which has no size for them, and before any
+    launch; the same call with a bad argument is invalid."""
+    lib = _lib.core()
+    assert lib.w8a8_attention_pages_workspace_size(n_seq, T, n_head, n_kv, max_ctx, n_shared) == 0
+    c = _pages(n_slot=8192, n_layer=1, n_kv_head=n_kv, page_stride=n_kv * 16 * 64)
+    d = n_head * 64
+
+    def call(ws, size, layer=0):
+        return lib.w8a8_attention_pages(c, layer, P, d, n_seq, T, None, max_ctx, P, n_shared,
+                                        n_head, 64, P, d, ws, size, None)
+    assert call(None, 0) == UNSUPPORTED and call(P, 1 << 40) == UNSUPPORTED
+    assert call(P, 1 << 40, layer=1) == INVALID
+
+
+def test_a_missing_or_small_workspace_is_invalid():
+    lib = _lib.core()
+    size = lib.w8a8_attention_pages_workspace_size(2, 1, 3, 3, 4096, 0)
+    assert size > 16
+    for ws, n in ((None, size), (P, size - 1), (P + 8, size)):
+        assert lib.w8a8_attention_pages(_pages(), 0, P, 192, 2, 1, None, 4096, None, 0, 3, 64, P,
+                                        192, ws, n, None) == INVALID
+
+
 def _cpu_cache(**kw):
     t = dict(K=torch.zeros(8, 2, 3, 16, 64, dtype=torch.bfloat16),
              V=torch.zeros(8, 2, 3, 16, 64, dtype=torch.bfloat16),

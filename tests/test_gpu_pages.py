@@ -794,6 +794,14 @@ def test_front_end_refusals(cuda):
     assert c.n_ctx.tolist() == [0, 0]
 
 
+def test_a_call_of_too_many_pieces_is_unsupported(cuda):
+    c, _ = make(cuda, 8, 64, 4)
+    Q = torch.zeros(64, 192, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(_lib.W8A8Error) as e:
+        ops.attention_pages(Q, c, 0, 3, max_ctx=1 << 30)
+    assert e.value.status == _lib.W8A8_ERR_UNSUPPORTED
+
+
 def test_the_slot_cache_attention_agrees(cuda):
     """The framework's path over both caches: the packed QKV projection writes new
     rows into the slot cache and, through pages_write, into pages; decode attention
