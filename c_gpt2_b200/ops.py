@@ -491,9 +491,10 @@ def attention_pages(Q, cache, layer, n_head, T=1, n_new=None, max_ctx=None, shar
                     n_shared=0, out=None, workspace=None):
     """Attention of the T newest positions of each sequence over its pages: rows
     b*T + t of Q [n_seq*T, n_head*64] for t < n_new[b] (default: all T; the other
-    rows of the output are left as they were). The first n_shared positions are
-    read, once for the batch, from shared_pages (int32, device); max_ctx (default:
-    what the table holds) bounds every length."""
+    rows of the output are left as they were). The first n_shared positions of every
+    sequence with new ones are read, once for the batch, from shared_pages (int32,
+    device; a copy of the table row of one that holds them); max_ctx (default: what
+    the table holds) bounds every length."""
     dev = _device_of(cache)
     d = n_head * 64
     n_seq = Q.shape[0] // T if T > 0 else 0

@@ -6,8 +6,14 @@ Sequences that go on from one prompt hold its pages once. ``ops.pages_extend``,
 
     pos0 = ops.pages_extend(cache, n_new)                  # once a step
     ops.pages_write(cache, layer, K, V, pos0)              # each layer
-    O = ops.attention_pages(Q, cache, layer, n_head, max_ctx=...,
-                            shared_pages=cache.table[0], n_shared=...)
+    O = ops.attention_pages(Q, cache, layer, n_head, n_new=n_new, max_ctx=...,
+                            shared_pages=prefix, n_shared=...)
+
+with n_new 1 for the slots that go on and 0 for those that have ended, and
+``prefix = cache.table[s].clone()`` of a slot s that holds the prompt, taken after
+the fork and again after each ``pages_compact`` (the row itself is emptied when
+the slot is freed). Sequences of several prompts: a call for each, with n_new 0
+for the others' sequences, into one ``out``.
 """
 from __future__ import annotations
 

@@ -292,8 +292,8 @@ typedef struct {
  * grows by it, new pages join table and refs. pos0[s] (device, [n_slot])
  * receives the first new position, W8A8_PAGES_NONE where n_new[s] <= 0, or
  * W8A8_PAGES_REFUSED where the slot was left as it was: its table row is too
- * short, or the free pages do not cover the pages that it and the slots before
- * it ask for. */
+ * short, or it needs a page and the free pages do not cover those that it and the
+ * slots before it ask for. */
 int w8a8_pages_extend(const w8a8_pages *c, const int32_t *n_new, int32_t *pos0, void *stream);
 
 /* Rows of a padded batch into the pages of one layer: row m = b*T + t of Kn and
@@ -346,14 +346,19 @@ int w8a8_pages_copy(const gpt2_bf16_t *Ksrc, const gpt2_bf16_t *Vsrc, int64_t sr
  *   sums and accumulators; the weights are rounded to bf16 for the product with V.
  * A row with end <= 0 is written as zeros; rows t >= n_new[b] are left as they
  * were. Positions below n_shared (a multiple of page, at most max_ctx) are read
- * from the n_shared / page pages shared_pages (device), for every sequence, and
- * the table's entries for them are not read: with sequences forked from one
- * prompt, any one's table row. Rows of pages that no query attends may hold
- * anything; a value that is not finite at a position that some query attends
+ * from the n_shared / page pages shared_pages (device), for every sequence with
+ * n_new[b] > 0, and the table's entries for them are not read. With sequences
+ * forked from one prompt that is a copy of any one's table row: the row itself is
+ * emptied when its slot is freed, and w8a8_pages_compact renames the pages, after
+ * which the copy is made anew. Sequences that do not begin with these pages are
+ * left out by n_new[b] = 0, as are slots that have ended; a batch behind several
+ * prompts is a call for each, into one O. Rows of pages that no query attends may
+ * hold anything; a value that is not finite at a position that some query attends
  * may reach every query of the call that shares its key head.
  * max_ctx bounds every n_ctx[b] (<= 2^30). The workspace (any contents; calls
  * that share one must not overlap on the GPU) is sized with
- * w8a8_attention_pages_workspace_size, 0 for sizes that are refused; 16-byte
+ * w8a8_attention_pages_workspace_size, 0 for sizes that are refused; smaller sizes
+ * can need more, so that one for several calls is their maximum. 16-byte
  * aligned Q and workspace, ldq % 8 == 0, O 4-byte aligned, ldo even;
  * n_head % n_kv_head == 0, head_dim 64, n_seq*T*n_head <= 2^30. Calls of some
  * 2^31 pieces of 16 rows x 64 keys or, where the kernels take 256 rows of one

@@ -834,6 +834,61 @@ def test_the_slot_cache_attention_agrees(cuda):
     assert (err <= (2.0 ** -8 * (2 * smax + 6)) * A).all()
 
 
+@pytest.mark.parametrize("blocks", [2, 60])
+def test_two_prompts_in_one_batch(cuda, blocks):
+    """Samples of two prompts in turn: a call for each prompt, the others' sequences left
+    out by n_new, into one output. Then the slots that the prompts came in by end, and the
+    pool is compacted: the rest go on behind copies of a live slot's row."""
+    G, H, page, n_seq = 4, 8, 32, 12
+    n_layer, lens = 1, [page * blocks + 3, page * (blocks - 1)]
+    c, _ = make(cuda, 4 * blocks + 40, n_seq, blocks + 4, n_layer, G, page, seed=5)
+    g = torch.Generator(device=cuda).manual_seed(6)
+    held = [None] * n_seq
+
+    def rows(n):
+        return torch.randn(n, G * 64, generator=g, device=cuda).bfloat16()
+
+    def add(n_new):
+        T = max(n_new)
+        K, V = rows(n_seq * T), rows(n_seq * T)
+        pos0 = ops.pages_extend(c, i32(n_new))
+        assert (pos0 >= -1).all()
+        ops.pages_write(c, 0, K, V, pos0, T=T, n_new=i32(n_new))
+        for b, n in enumerate(n_new):
+            if n:
+                new = [x[b * T:b * T + n].view(n, G, 64) for x in (K, V)]
+                held[b] = [torch.cat(x) for x in zip(held[b], new)] if held[b] else new
+
+    def step(live, holder):
+        add(live)
+        Q = torch.randn(n_seq, H * 64, generator=g, device=cuda).bfloat16()
+        out = torch.full_like(Q, 7.0)
+        for i in range(2):
+            whole = lens[i] // page
+            prefix = c.table[holder[i], :whole].clone()
+            ops.attention_pages(Q, c, 0, H, n_new=i32([v * (b % 2 == i) for b, v in enumerate(live)]),
+                                max_ctx=page * (blocks + 2), shared_pages=prefix,
+                                n_shared=whole * page, out=out)
+        q64 = Q.double().cpu().numpy().reshape(n_seq, 1, H, 64)
+        want = [po.attention(q64[b], *(x.double().cpu().numpy() for x in held[b] or
+                                       [torch.zeros(0, G, 64)] * 2), live[b]) for b in range(n_seq)]
+        check(out, want, 1, H, live)
+
+    add(lens + [0] * (n_seq - 2))
+    src, dst = [b % 2 for b in range(2, n_seq)], list(range(2, n_seq))
+    assert ops.pages_fork(c, i32(src), i32(dst)).tolist() == [0] * (n_seq - 2)
+    for a, b in zip(src, dst):
+        held[b] = held[a]
+    step([1] * n_seq, [0, 1])
+    ops.pages_free(c, i32([0, 1, 6]))
+    held[0] = held[1] = held[6] = None
+    live = [0, 0, 1, 1, 1, 1, 0, 1, 1, 1, 1, 1]
+    step(live, [2, 3])
+    ops.pages_compact(c)
+    step(live, [4, 11])
+    assert c.n_ctx.tolist() == [v * (lens[b % 2] + 3) for b, v in enumerate(live)]
+
+
 def test_a_serving_run(cuda):
     """Two prompts of different lengths (a padded batch) through the packed QKV
     projection into pages; three samples of each, decoded step by step behind the
