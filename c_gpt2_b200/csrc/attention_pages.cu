@@ -496,10 +496,11 @@ __device__ __forceinline__ void mma_stage(MmaState &w, uint32_t kb, uint32_t vb,
 // copy rate. The warps work alone, with no barrier between them, each with two
 // 64-key stages that it fills itself by TMA (128-byte swizzle), one ahead, across
 // the ends of items (four warps with three stages: 31 us where six with two take
-// 25.5, seven 24.5). Measured, 64 sequences of 20 heads, nothing shared: 5.4 TB/s
-// with up to 4096 positions each (683 MB, 125 us; without the arithmetic 118), but
-// 29 us with up to 512 (85 MB): some 4 us until the first keys arrive, 4 for the
-// join, and SMs that get their bytes up to a fifth later than the average.
+// 25.5, seven 24.5). Measured, 64 sequences of 20 heads, nothing shared: 5.7 TB/s
+// with up to 4096 positions each (645 to 726 MB by the lengths drawn, 114 to 128 us;
+// 6 % less without the arithmetic), but 28 to 30 us with up to 512 (81 to 91 MB):
+// some 4 us until the first keys arrive, 4 for the join, and SMs that get their
+// bytes up to a quarter later than the average.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(kMmaWarps * 32, 1)
     attention_pages_mma_kernel(const __grid_constant__ CUtensorMap tmK,

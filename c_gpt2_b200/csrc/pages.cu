@@ -269,8 +269,9 @@ __global__ void __launch_bounds__(kBookThreads)
 // that the last pages hold: a CTA takes a piece of a page (four 16-byte
 // units a thread, of both pools in turn) and copies it for its share of the list,
 // keeping what it read while the source stays the same: for the forks of one
-// sequence nothing but the writes is left (63 forks of 19 rows, 36 layers of 20
-// heads, 220 MB: 53 us, 4.1 TB/s, as fast as memory is filled).
+// sequence the writes are left, and the reads of each entry's status, length and
+// pages, one after the other, which its stores wait for (63 forks of 19 rows, 36
+// layers of 20 heads, 220 MB: 52 us, 4.2 TB/s; a plain fill of as much takes 34).
 __global__ void __launch_bounds__(256)
     pages_fork_rows_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n,
                            const int32_t *status) {
